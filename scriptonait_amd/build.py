@@ -26,19 +26,20 @@ CSRC = PKG_DIR / "csrc"
 LIB_NAME = "libllmhip_sampler.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = ["sampler_kernels.hip", "vocab_full.hip", "vocab_plain.hip", "fast_nch8.hip", "fast_nch_small.hip", "fast_counts.hip", "fast_counts8.hip",
-           "fast_counts_small.hip", "tied_head.hip", "bench_floor.hip", "stream_topk.hip", "stream_topk_bigk.hip", "stream_topk_refine.hip", "sampler_api.hip", "scck_reader.cpp"]
+           "fast_counts_small.hip", "tied_head.hip", "bench_floor.hip", "stream_topk.hip", "stream_topk_bigk.hip", "stream_topk_refine.hip", "sampler_api.hip", "scck_reader.cpp",
+           "kv_plan.hip", "kv_append.hip", "kv_attend.hip", "kv_api.hip"]
 ARCH = "gfx950"
 
 
 def source_hash() -> str:
     """SHA-256 (first 16 hex digits) over the library's sources and the
-    header: the identity of a build, which measured profile figures name so
+    headers: the identity of a build, which measured profile figures name so
     that bench.py can tell whether they belong to the library it runs."""
     import hashlib
 
     h = hashlib.sha256()
     files = (sorted(CSRC.glob("*.h")) + sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("*.cpp"))
-             + [PKG_DIR.parent / "include" / "llmhip_sampler.h"])
+             + sorted((PKG_DIR.parent / "include").glob("*.h")))
     for f in files:
         h.update(f.name.encode())
         h.update(f.read_bytes())

@@ -1,0 +1,255 @@
+// C entry points of the paged key-value cache (declared in
+// include/llmhip_kv.h): what the host can check, and the launches. Arguments
+// are checked before the context, so a wrong call says what is wrong with it
+// also where there is no device.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+
+#include "ctx_info.h"
+#include "device_scope.h"
+#include "kv_args.h"
+
+using namespace llmhip;
+
+namespace {
+
+int arg_fail(const char* what) {
+  set_last_error(what);
+  return LLMHIP_ERR_INVALID_ARGUMENT;
+}
+int unsupported(const char* what) {
+  set_last_error(what);
+  return LLMHIP_ERR_UNSUPPORTED;
+}
+int launched(hipError_t e, const char* what) {
+  if (e == hipSuccess) return LLMHIP_OK;
+  char buf[256];
+  snprintf(buf, sizeof buf, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
+  set_last_error(buf);
+  return e == hipErrorOutOfMemory ? LLMHIP_ERR_OUT_OF_MEMORY : LLMHIP_ERR_HIP;
+}
+
+#define ARG(cond, what) \
+  if (!(cond)) return arg_fail(what)
+#define SUPPORTED(cond, what) \
+  if (!(cond)) return unsupported(what)
+
+constexpr size_t kMaxInt = 0x7fffffff;
+constexpr size_t kMaxBatch = 65535;
+constexpr size_t kMaxHeads = 65535;
+
+uint32_t size_of(uint32_t dtype) { return dtype == LLMHIP_F32 ? 4u : dtype == LLMHIP_E4M3 ? 1u : 2u; }
+
+// Whether every row of an operand starts on `bytes`.
+bool rows_on(const void* p, const int64_t* strides, int n, uint32_t elem, uint32_t bytes) {
+  if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
+  for (int i = 0; i < n; ++i)
+    if ((uint64_t)strides[i] * elem % bytes) return false;
+  return true;
+}
+
+int check_cache(const llmhip_kv_cache* c) {
+  ARG(c, "cache is null");
+  ARG(c->dtype <= LLMHIP_E4M3, "unknown cache dtype");
+  ARG(c->k_pool && c->v_pool, "k_pool and v_pool are required");
+  ARG((c->dtype == LLMHIP_E4M3) == (c->k_scale != nullptr) && (c->dtype == LLMHIP_E4M3) == (c->v_scale != nullptr),
+      "k_scale and v_scale go with an E4M3 cache, and only with one");
+  ARG(c->pages >= 1 && c->page >= 1 && c->heads >= 1, "pages, page and heads must be at least 1");
+  SUPPORTED(c->pages <= kMaxInt && c->page <= kMaxInt && c->heads <= kMaxHeads, "pages, page or heads too large");
+  SUPPORTED(c->head_dim >= 8 && c->head_dim <= kMaxHeadDim && c->head_dim % 8 == 0,
+            "head_dim must be a multiple of 8 up to 256");
+  for (int i = 0; i < 3; ++i) ARG(c->k_stride[i] >= 0 && c->v_stride[i] >= 0, "pool strides must not be negative");
+  const uint32_t elem = size_of(c->dtype), bytes = elem == 1 ? 8 : 16;
+  SUPPORTED(rows_on(c->k_pool, c->k_stride, 3, elem, bytes) && rows_on(c->v_pool, c->v_stride, 3, elem, bytes),
+            "pool rows must be aligned to 16 bytes (8 for E4M3)");
+  return LLMHIP_OK;
+}
+
+int check_dtype(const llmhip_kv_cache* c, uint32_t dtype) {
+  ARG(dtype <= LLMHIP_F16, "dtype must be F32, BF16 or F16");
+  ARG(dtype == c->dtype || c->dtype == LLMHIP_E4M3, "dtype is neither the cache's nor beside an E4M3 cache");
+  return LLMHIP_OK;
+}
+
+int check_table(size_t table_pages, size_t table_ld, size_t page) {
+  ARG(table_ld >= table_pages, "table_ld < table_pages");
+  SUPPORTED(table_pages <= kMaxInt && (table_pages + 1) * page <= kMaxInt, "table_pages * page must be below 2^31");
+  return LLMHIP_OK;
+}
+
+#define TRY(expr)                       \
+  do {                                  \
+    const int st_ = (expr);             \
+    if (st_ != LLMHIP_OK) return st_;   \
+  } while (0)
+
+#define ON_DEVICE(info)                                                    \
+  ARG(ctx, "ctx is null");                                                 \
+  const CtxInfo info = ctx_info(ctx);                                      \
+  Device scope(info.device);                                               \
+  if (!scope.ok) return launched(hipErrorInvalidDevice, "hipSetDevice")
+
+void set_pools(const llmhip_kv_cache* c, const void** pool, const float** scale, int64_t (*stride)[3]) {
+  pool[0] = c->k_pool;
+  pool[1] = c->v_pool;
+  scale[0] = c->k_scale;
+  scale[1] = c->v_scale;
+  memcpy(stride[0], c->k_stride, sizeof c->k_stride);
+  memcpy(stride[1], c->v_stride, sizeof c->v_stride);
+}
+
+}  // namespace
+
+extern "C" {
+
+int llmhip_kv_plan(llmhip_ctx* ctx, size_t pages, size_t page, int32_t* ring, const int32_t* free_state, size_t R,
+                   const int32_t* lens, const int32_t* new_tokens, const int32_t* release, int32_t* table,
+                   size_t table_pages, size_t table_ld, int32_t* out_lens, int32_t* granted, int32_t* start, size_t T,
+                   int64_t* slots, int32_t* positions, int32_t* out_free_state, void* stream) {
+  ARG(pages >= 1 && page >= 1, "pages and page must be at least 1");
+  SUPPORTED(pages <= kMaxInt && page <= kMaxInt, "pages or page too large");
+  ARG(ring && free_state && out_free_state, "ring, free_state and out_free_state are required");
+  ARG(R == 0 || (lens && out_lens && granted), "lens, out_lens and granted are required");
+  ARG(R == 0 || table_pages == 0 || table, "table is null");
+  ARG(start, "start is null");
+  ARG(T == 0 || (slots && positions), "slots and positions are required");
+  SUPPORTED(R <= kMaxInt - 1024 && T <= kMaxInt - 1024, "R or T too large");
+  TRY(check_table(table_pages, table_ld, page));
+  ON_DEVICE(info);
+  PlanArgs a{};
+  a.ring = ring;
+  a.free_state = free_state;
+  a.out_free_state = out_free_state;
+  a.lens = lens;
+  a.new_tokens = new_tokens;
+  a.release = release;
+  a.table = table;
+  a.out_lens = out_lens;
+  a.granted = granted;
+  a.start = start;
+  a.slots = slots;
+  a.positions = positions;
+  a.table_ld = table_ld;
+  a.pages = (uint32_t)pages;
+  a.page = (uint32_t)page;
+  a.table_pages = (uint32_t)table_pages;
+  a.R = (uint32_t)R;
+  a.T = (uint32_t)T;
+  a.by_page = FastDiv::of(a.page);
+  a.status = info.status;
+  return launched(launch_kv_plan(a, static_cast<hipStream_t>(stream)), "llmhip_kv_plan");
+}
+
+int llmhip_kv_append(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dtype, size_t T, const void* k,
+                     const int64_t k_stride[2], const void* v, const int64_t v_stride[2], const int64_t* slots,
+                     size_t q_heads, const void* q, const int64_t q_stride[2], void* out_q,
+                     const int64_t out_q_stride[2], const int32_t* positions, const llmhip_rope* rope, void* stream) {
+  TRY(check_cache(cache));
+  TRY(check_dtype(cache, dtype));
+  ARG((q == nullptr) == (out_q == nullptr) && (q == nullptr) == (q_heads == 0), "q, out_q and q_heads go together");
+  ARG(!rope || rope->dims == 0 || rope->freqs, "rope->freqs is null");
+  ARG(!rope || rope->style <= LLMHIP_ROPE_NEIGHBOURS, "unknown rope style");
+  ARG(!rope || (rope->dims % 2 == 0 && rope->dims <= cache->head_dim), "rope->dims must be even and at most head_dim");
+  const uint32_t dims = rope ? rope->dims : 0u;
+  SUPPORTED(T <= kMaxInt - 1024 && q_heads <= kMaxHeads, "T or q_heads too large");
+  if (T == 0) return LLMHIP_OK;
+  ARG(k && v && slots && k_stride && v_stride, "k, v, slots and their strides are required");
+  ARG(!q || (q_stride && out_q_stride), "q_stride and out_q_stride are required");
+  ARG(!dims || positions, "positions are required with rope");
+  // The widest access that the rows' starts and the pairs' places allow: 8
+  // values (16 bytes of 16-bit types), 4, or single ones.
+  const uint32_t elem = size_of(dtype), kv_elem = size_of(cache->dtype), dim = cache->head_dim;
+  const bool neighbours = rope && rope->style == LLMHIP_ROPE_NEIGHBOURS;
+  uint32_t vec = 8;
+  for (; vec > 1; vec = vec == 8 ? 4 : 1) {
+    const uint32_t bytes = vec * elem, kv_bytes = vec * kv_elem;
+    if (dims % (2 * vec) || (dim - dims) % (2 * vec)) continue;
+    if (!rows_on(k, k_stride, 2, elem, bytes) || !rows_on(v, v_stride, 2, elem, bytes)) continue;
+    if (q && (!rows_on(q, q_stride, 2, elem, bytes) || !rows_on(out_q, out_q_stride, 2, elem, bytes))) continue;
+    if (rows_on(cache->k_pool, cache->k_stride, 3, kv_elem, kv_bytes) &&
+        rows_on(cache->v_pool, cache->v_stride, 3, kv_elem, kv_bytes))
+      break;
+  }
+  ON_DEVICE(info);
+  AppendArgs a{};
+  a.x[0] = q;
+  a.x[1] = k;
+  a.x[2] = v;
+  a.out_q = out_q;
+  set_pools(cache, const_cast<const void**>(a.pool), a.scale, a.pool_stride);
+  if (q) memcpy(a.x_stride[0], q_stride, sizeof a.x_stride[0]);
+  memcpy(a.x_stride[1], k_stride, sizeof a.x_stride[1]);
+  memcpy(a.x_stride[2], v_stride, sizeof a.x_stride[2]);
+  if (q) memcpy(a.oq_stride, out_q_stride, sizeof a.oq_stride);
+  a.slots = slots;
+  a.positions = positions;
+  a.T = (uint32_t)T;
+  a.q_heads = (uint32_t)q_heads;
+  a.heads = cache->heads;
+  a.dim = dim;
+  a.dims = dims;
+  a.pages = cache->pages;
+  a.page = cache->page;
+  a.status = info.status;
+  if (dims) memcpy(a.freqs, rope->freqs, dims / 2 * sizeof(double));
+  return launched(launch_kv_append(a, dtype, cache->dtype, neighbours, vec, static_cast<hipStream_t>(stream)),
+                  "llmhip_kv_append");
+}
+
+int llmhip_kv_attend_workspace(llmhip_ctx* ctx, const llmhip_kv_cache* cache, size_t q_heads, size_t* bytes) {
+  ARG(bytes, "bytes is null");
+  TRY(check_cache(cache));
+  ARG(q_heads >= 1 && q_heads % cache->heads == 0, "q_heads must be a multiple of the cache's heads");
+  SUPPORTED(q_heads <= kMaxHeads, "q_heads too large");
+  ARG(ctx, "ctx is null");
+  *bytes = 256;
+  return LLMHIP_OK;
+}
+
+int llmhip_kv_attend(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dtype, size_t B, size_t q_heads,
+                     const void* q, const int64_t q_stride[2], const int32_t* table, size_t table_pages,
+                     size_t table_ld, const int32_t* lens, size_t window, float scale, void* out,
+                     const int64_t out_stride[2], float* out_lse, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  TRY(check_cache(cache));
+  TRY(check_dtype(cache, dtype));
+  ARG(cache->dtype != LLMHIP_E4M3 || dtype != LLMHIP_F32, "dtype beside an E4M3 cache is BF16 or F16");
+  ARG(q_heads >= 1 && q_heads % cache->heads == 0, "q_heads must be a multiple of the cache's heads");
+  SUPPORTED(q_heads <= kMaxHeads && B <= kMaxBatch, "B or q_heads too large");
+  TRY(check_table(table_pages, table_ld, cache->page));
+  if (B == 0) return LLMHIP_OK;
+  ARG(q && out && lens && q_stride && out_stride, "q, out, lens and their strides are required");
+  ARG(table || table_pages == 0, "table is null");
+  ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be given, aligned to 16 bytes");
+  size_t need = 0;
+  TRY(llmhip_kv_attend_workspace(ctx, cache, q_heads, &need));
+  ARG(workspace_bytes >= need, "workspace is smaller than llmhip_kv_attend_workspace says");
+  ON_DEVICE(info);
+  AttendArgs a{};
+  a.q = q;
+  a.out = out;
+  a.lse = out_lse;
+  set_pools(cache, a.pool, a.scale, a.pool_stride);
+  a.table = table;
+  a.lens = lens;
+  memcpy(a.q_stride, q_stride, sizeof a.q_stride);
+  memcpy(a.out_stride, out_stride, sizeof a.out_stride);
+  a.table_ld = table_ld;
+  a.workspace = static_cast<float*>(workspace);
+  a.B = (uint32_t)B;
+  a.q_heads = (uint32_t)q_heads;
+  a.heads = cache->heads;
+  a.dim = cache->head_dim;
+  a.pages = cache->pages;
+  a.page = cache->page;
+  a.table_pages = (uint32_t)table_pages;
+  a.window = window < kMaxInt ? (uint32_t)window : 0u;
+  a.score_scale = scale;
+  a.by_page = FastDiv::of(a.page);
+  a.status = info.status;
+  return launched(launch_kv_attend(a, dtype, cache->dtype, static_cast<hipStream_t>(stream)), "llmhip_kv_attend");
+}
+
+}  // extern "C"

@@ -1,0 +1,72 @@
+// Arguments of the paged key-value cache's kernels, passed by value.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/llmhip_kv.h"
+#include "kv_index.h"
+
+namespace llmhip {
+
+constexpr uint32_t kMaxHeadDim = 256;
+
+struct PlanArgs {
+  int32_t* ring;
+  const int32_t* free_state;
+  int32_t* out_free_state;
+  const int32_t* lens;
+  const int32_t* new_tokens;  // nullable
+  const int32_t* release;     // nullable
+  int32_t* table;
+  int32_t* out_lens;
+  int32_t* granted;
+  int32_t* start;
+  int64_t* slots;
+  int32_t* positions;
+  uint64_t table_ld;
+  uint32_t pages, page, table_pages, R, T;
+  FastDiv by_page;
+  uint32_t* status;
+};
+
+struct AppendArgs {
+  const void* x[3];  // queries, keys, values
+  void* out_q;
+  void* pool[2];
+  const float* scale[2];  // E4M3: one for each head
+  int64_t x_stride[3][2];
+  int64_t oq_stride[2];
+  int64_t pool_stride[2][3];
+  const int64_t* slots;
+  const int32_t* positions;
+  uint32_t T, q_heads, heads, dim, dims, pages, page;
+  FastDiv by_token, by_row;  // units of a token, units of a head row
+  uint32_t tokens_per_group;
+  uint32_t* status;
+  double freqs[kMaxHeadDim / 2];
+};
+
+struct AttendArgs {
+  const void* q;
+  void* out;
+  float* lse;  // nullable
+  const void* pool[2];
+  const float* scale[2];
+  const int32_t* table;
+  const int32_t* lens;
+  int64_t q_stride[2], out_stride[2];
+  int64_t pool_stride[2][3];
+  uint64_t table_ld;
+  float* workspace;
+  uint32_t B, q_heads, heads, dim, pages, page, table_pages, window;
+  float score_scale;
+  FastDiv by_page;
+  uint32_t* status;
+};
+
+hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s);
+hipError_t launch_kv_append(const AppendArgs& a, uint32_t dtype, uint32_t kv_dtype, bool neighbours, uint32_t vec,
+                            hipStream_t s);
+hipError_t launch_kv_attend(const AttendArgs& a, uint32_t dtype, uint32_t kv_dtype, hipStream_t s);
+
+}  // namespace llmhip

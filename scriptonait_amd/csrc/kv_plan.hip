@@ -1,0 +1,180 @@
+// Pages, slots and positions for the tokens of the next step
+// (llmhip_kv_plan).
+//
+// Requests are served in order, so what request r gets follows from sums
+// over the requests before it: of their tokens, of the pages that they need
+// and of the pages that they give back. One workgroup forms the three prefix
+// sums, 1024 requests at a time, in 64 bits; each token of the chunk then
+// finds its request by bisection of the sums in LDS.
+#include "kv_args.h"
+#include "wave_ops.h"
+
+namespace llmhip {
+namespace {
+
+constexpr uint32_t kThreads = 1024;
+constexpr uint32_t kWaves = kThreads / 64;
+
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ uint64_t dpp0_u64(uint64_t x) {
+  return ((uint64_t)dpp0<CTRL, ROW_MASK>((uint32_t)(x >> 32)) << 32) | dpp0<CTRL, ROW_MASK>((uint32_t)x);
+}
+
+// wave_incl_scan in 64 bits.
+__device__ __forceinline__ uint64_t wave_incl_scan_u64(uint64_t x) {
+  x += dpp0_u64<0x111>(x);
+  x += dpp0_u64<0x112>(x);
+  x += dpp0_u64<0x114>(x);
+  x += dpp0_u64<0x118>(x);
+  x += dpp0_u64<0x142, 0xa>(x);
+  x += dpp0_u64<0x143, 0xc>(x);
+  return x;
+}
+
+// Inclusive prefix sum over the workgroup and its total. `waves`: kWaves
+// words that no other sum uses until the next barrier.
+__device__ __forceinline__ uint64_t group_scan(uint64_t x, uint64_t* waves, uint64_t& total) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+  x = wave_incl_scan_u64(x);
+  if (lane == 63u) waves[wave] = x;
+  __syncthreads();
+  const uint64_t sums = wave_incl_scan_u64(lane < kWaves ? waves[lane] : 0u);
+  total = readlane_u64(sums, kWaves - 1u);
+  return x + (wave ? readlane_u64(sums, wave - 1u) : 0u);
+}
+
+__global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
+  __shared__ uint64_t s_waves[3][kWaves];
+  __shared__ uint32_t s_end[kThreads];    // tokens asked for up to and with each request, at most T + 1
+  __shared__ uint32_t s_begin[kThreads];  // and before it
+  __shared__ uint32_t s_base[kThreads];   // its tokens before this call
+  __shared__ uint32_t s_first[kThreads];  // where its new pages start in the ring
+  __shared__ uint32_t s_took[kThreads];   // how many they are
+  __shared__ uint32_t s_back[kThreads];   // pages that it gives back
+  __shared__ uint32_t s_put[kThreads];    // where they go in the ring
+  __shared__ uint32_t s_ok[kThreads];
+  const uint32_t tid = threadIdx.x;
+  const uint64_t cap = (uint64_t)a.table_pages * a.page;
+  const uint32_t most = cap > 0x7fffffffu ? 0x7fffffffu : (uint32_t)cap;
+  bool bad = false;
+  uint32_t head = (uint32_t)a.free_state[0], count = (uint32_t)a.free_state[1];
+  if (head >= a.pages || count > a.pages) {
+    bad = true;
+    head = 0u;
+    count = 0u;
+  }
+  uint64_t asked = 0, needed = 0, returned = 0, taken = 0;
+  if (tid == 0u) a.start[0] = 0;
+  for (uint32_t r0 = 0; r0 < a.R; r0 += kThreads) {
+    const uint32_t r = r0 + tid, m = min(kThreads, a.R - r0);
+    uint32_t base = 0, back = 0;
+    uint64_t n = 0;
+    if (r < a.R) {
+      const uint32_t len = clamp_len(a.lens[r], most, bad);
+      const bool gone = a.release && a.release[r] != 0;
+      base = gone ? 0u : len;
+      back = gone ? a.by_page.div(len + a.page - 1u) : 0u;
+      if (a.new_tokens) {
+        const int32_t want = a.new_tokens[r];
+        bad = bad || want < 0;
+        n = want < 0 ? 0u : (uint32_t)want;
+      } else {
+        n = gone ? 0u : 1u;
+      }
+    }
+    uint64_t n_sum, need_sum, back_sum;
+    const uint64_t end = asked + group_scan(n, s_waves[0], n_sum);
+    const uint64_t put = returned + group_scan(back, s_waves[1], back_sum) - back;
+    const bool fits = r < a.R && base + n <= cap && end <= a.T;
+    const uint32_t have = a.by_page.div(base + a.page - 1u);
+    const uint32_t need = fits ? a.by_page.div(base + (uint32_t)n + a.page - 1u) - have : 0u;
+    const uint64_t upto = needed + group_scan(need, s_waves[2], need_sum);
+    const bool ok = fits && (need == 0u || upto <= count);
+    s_end[tid] = (uint32_t)min(end, (uint64_t)a.T + 1u);
+    s_begin[tid] = (uint32_t)min(end - n, (uint64_t)a.T + 1u);
+    s_base[tid] = base;
+    s_first[tid] = (uint32_t)((head + (upto - need)) % a.pages);
+    s_took[tid] = ok ? need : 0u;
+    s_back[tid] = back;
+    s_put[tid] = (uint32_t)((head + count + put) % a.pages);
+    s_ok[tid] = ok;
+    if (r < a.R) {
+      a.out_lens[r] = (int32_t)(base + (ok ? (uint32_t)n : 0u));
+      a.granted[r] = ok ? (int32_t)n : 0;
+      a.start[r + 1u] = (int32_t)(uint32_t)end;
+    }
+    __syncthreads();
+
+    // Released pages, read before a new page may take their place in the table.
+    for (uint32_t i = tid >> 6; i < m; i += kWaves) {
+      int32_t* row = a.table + (uint64_t)(r0 + i) * a.table_ld;
+      for (uint32_t p = tid & 63u; p < s_back[i]; p += 64u) a.ring[((uint64_t)s_put[i] + p) % a.pages] = row[p];
+    }
+    __syncthreads();
+
+    const uint32_t lo = (uint32_t)min(asked, (uint64_t)a.T), hi = (uint32_t)min(asked + n_sum, (uint64_t)a.T);
+    for (uint32_t t = lo + tid; t < hi; t += kThreads) {
+      uint32_t i = 0, above = m;  // the first request whose sum passes t
+      while (i < above) {
+        const uint32_t mid = (i + above) >> 1;
+        if (s_end[mid] > t) above = mid;
+        else i = mid + 1u;
+      }
+      int64_t slot = -1;
+      uint32_t pos = 0;
+      if (s_ok[i]) {
+        pos = s_base[i] + (t - s_begin[i]);
+        const uint32_t p = a.by_page.div(pos), have_i = a.by_page.div(s_base[i] + a.page - 1u);
+        int32_t* entry = a.table + (uint64_t)(r0 + i) * a.table_ld + p;
+        int32_t id;
+        if (p >= have_i) {
+          id = a.ring[((uint64_t)s_first[i] + (p - have_i)) % a.pages];
+          if (pos == p * a.page) *entry = id;  // a page's first token enters it
+        } else {
+          id = *entry;
+        }
+        if ((uint32_t)id < a.pages) slot = (int64_t)id * a.page + (pos - p * a.page);
+        else bad = true;
+      }
+      a.slots[t] = slot;
+      a.positions[t] = (int32_t)pos;
+    }
+    // The requests that got pages are the first of those that need some, so
+    // the largest of their sums is what the chunk took.
+    uint64_t mine = ok && need ? upto : 0u;
+#pragma unroll
+    for (uint32_t off = 32; off; off >>= 1) {
+      const uint64_t other =
+          ((uint64_t)__shfl_xor((uint32_t)(mine >> 32), off, 64) << 32) | __shfl_xor((uint32_t)mine, off, 64);
+      mine = max(mine, other);
+    }
+    if ((tid & 63u) == 0u) s_waves[0][tid >> 6] = mine;
+    __syncthreads();
+    for (uint32_t w = 0; w < kWaves; ++w) taken = max(taken, s_waves[0][w]);
+    asked += n_sum;
+    needed += need_sum;
+    returned += back_sum;
+    __syncthreads();
+  }
+
+  for (uint32_t t = (uint32_t)min(asked, (uint64_t)a.T) + tid; t < a.T; t += kThreads) {
+    a.slots[t] = -1;
+    a.positions[t] = 0;
+  }
+  if (tid == 0u) {
+    const uint64_t left = count - taken + returned;
+    bad = bad || left > a.pages;  // pages came back that were free already
+    a.out_free_state[0] = (int32_t)((head + taken) % a.pages);
+    a.out_free_state[1] = (int32_t)min(left, (uint64_t)a.pages);
+  }
+  if (__any(bad) && (tid & 63u) == 0u) atomicOr(a.status, LLMHIP_KSTATUS_BAD_INDEX);
+}
+
+}  // namespace
+
+hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace llmhip

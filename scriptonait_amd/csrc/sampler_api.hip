@@ -10,6 +10,8 @@
 #include <mutex>
 #include <string>
 
+#include "ctx_info.h"
+#include "device_scope.h"
 #include "grow_buf.h"
 #include "sampler_common.h"
 
@@ -117,6 +119,12 @@ struct llmhip_ctx {
   bool host_word_set = false;  // a host call ended early: its flags may still be set
 };
 
+namespace llmhip {
+CtxInfo ctx_info(const llmhip_ctx* ctx) {
+  return {ctx->device, ctx->cus, static_cast<uint32_t*>(ctx->status.ptr) + kStatusDeviceWord};
+}
+}  // namespace llmhip
+
 namespace {
 
 // Device address of `scratch` on each device, looked up once per device.
@@ -144,18 +152,6 @@ uint32_t* noalloc_scratch(int device) {
   }
   return g_noalloc_ptr[device];
 }
-
-struct Device {
-  int prev = -1;
-  bool ok = false;
-  explicit Device(int dev) {
-    if (hipGetDevice(&prev) != hipSuccess) prev = -1;
-    ok = hipSetDevice(dev) == hipSuccess;
-  }
-  ~Device() {
-    if (prev >= 0) (void)hipSetDevice(prev);
-  }
-};
 
 int validate(size_t B, size_t V, size_t ld, const float* logits, const llmhip_params* params,
              const uint32_t* hist, const uint32_t* hist_offsets, const void* allowed,
