@@ -7,6 +7,8 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
+
 #include "ctx_info.h"
 #include "device_scope.h"
 #include "kv_args.h"
@@ -75,7 +77,7 @@ int check_dtype(const llmhip_kv_cache* c, uint32_t dtype) {
 
 int check_table(size_t table_pages, size_t table_ld, size_t page) {
   ARG(table_ld >= table_pages, "table_ld < table_pages");
-  SUPPORTED(table_pages <= kMaxInt && (table_pages + 1) * page <= kMaxInt, "table_pages * page must be below 2^31");
+  SUPPORTED(table_pages <= kMaxInt && (table_pages + 1) * page <= kMaxInt - 64, "table_pages * page must be below 2^31");
   return LLMHIP_OK;
 }
 
@@ -90,6 +92,21 @@ int check_table(size_t table_pages, size_t table_ld, size_t page) {
   const CtxInfo info = ctx_info(ctx);                                      \
   Device scope(info.device);                                               \
   if (!scope.ok) return launched(hipErrorInvalidDevice, "hipSetDevice")
+
+// How llmhip_kv_attend cuts its work: a workgroup takes a range of one block
+// of query heads, two workgroups a compute unit.
+struct AttendPlan {
+  uint32_t group, blocks, vheads, ranges, part_words;
+  AttendPlan(const llmhip_kv_cache* c, size_t q_heads, uint32_t cus) {
+    group = (uint32_t)q_heads / c->heads;
+    blocks = (group + 15u) / 16u;
+    vheads = blocks * c->heads;
+    ranges = std::min(std::max(2u * cus / vheads, 1u), kMaxRanges);
+    const uint32_t g = std::min(group, 16u);
+    part_words = (g * (c->head_dim + 2u) + 3u) / 4u * 4u;
+  }
+  size_t bytes() const { return ((size_t)kMaxSplitBatch + 4 + (size_t)ranges * vheads * 2 * part_words) * 4; }
+};
 
 void set_pools(const llmhip_kv_cache* c, const void** pool, const float** scale, int64_t (*stride)[3]) {
   pool[0] = c->k_pool;
@@ -204,7 +221,7 @@ int llmhip_kv_attend_workspace(llmhip_ctx* ctx, const llmhip_kv_cache* cache, si
   ARG(q_heads >= 1 && q_heads % cache->heads == 0, "q_heads must be a multiple of the cache's heads");
   SUPPORTED(q_heads <= kMaxHeads, "q_heads too large");
   ARG(ctx, "ctx is null");
-  *bytes = 256;
+  *bytes = AttendPlan(cache, q_heads, ctx_info(ctx).cus).bytes();
   return LLMHIP_OK;
 }
 
@@ -223,10 +240,9 @@ int llmhip_kv_attend(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
   ARG(q && out && lens && q_stride && out_stride, "q, out, lens and their strides are required");
   ARG(table || table_pages == 0, "table is null");
   ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be given, aligned to 16 bytes");
-  size_t need = 0;
-  TRY(llmhip_kv_attend_workspace(ctx, cache, q_heads, &need));
-  ARG(workspace_bytes >= need, "workspace is smaller than llmhip_kv_attend_workspace says");
   ON_DEVICE(info);
+  const AttendPlan plan(cache, q_heads, info.cus);
+  ARG(workspace_bytes >= plan.bytes(), "workspace is smaller than llmhip_kv_attend_workspace says");
   AttendArgs a{};
   a.q = q;
   a.out = out;
@@ -247,9 +263,24 @@ int llmhip_kv_attend(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
   a.table_pages = (uint32_t)table_pages;
   a.window = window < kMaxInt ? (uint32_t)window : 0u;
   a.score_scale = scale;
+  a.wide = rows_on(q, q_stride, 2, size_of(dtype), 16) && rows_on(out, out_stride, 2, size_of(dtype), 16);
+  a.group = plan.group;
+  a.blocks = plan.blocks;
+  a.vheads = plan.vheads;
+  a.ranges = B <= kMaxSplitBatch ? plan.ranges : 0u;
+  a.start_words = a.ranges ? (a.B + 1u + 3u) / 4u * 4u : 0u;
+  a.part_words = plan.part_words;
+  a.part_offset = kMaxSplitBatch + 4u;
   a.by_page = FastDiv::of(a.page);
+  a.by_dim = FastDiv::of(a.dim);
   a.status = info.status;
-  return launched(launch_kv_attend(a, dtype, cache->dtype, static_cast<hipStream_t>(stream)), "llmhip_kv_attend");
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool bf16 = dtype == LLMHIP_BF16;
+  hipError_t e;
+  if (cache->dtype == LLMHIP_E4M3) e = bf16 ? launch_attend_e4m3_bf16(a, s) : launch_attend_e4m3_f16(a, s);
+  else if (cache->dtype == LLMHIP_F32) e = launch_attend_f32(a, s);
+  else e = bf16 ? launch_attend_bf16(a, s) : launch_attend_f16(a, s);
+  return launched(e, "llmhip_kv_attend");
 }
 
 }  // extern "C"

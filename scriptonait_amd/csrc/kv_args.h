@@ -9,6 +9,10 @@
 namespace llmhip {
 
 constexpr uint32_t kMaxHeadDim = 256;
+// Attention: the ranges that a call's work is cut into, and the requests of a
+// call that is cut (their tiles' prefix sums live in LDS).
+constexpr uint32_t kMaxRanges = 1024;
+constexpr uint32_t kMaxSplitBatch = 2048;
 
 struct PlanArgs {
   int32_t* ring;
@@ -60,13 +64,23 @@ struct AttendArgs {
   float* workspace;
   uint32_t B, q_heads, heads, dim, pages, page, table_pages, window;
   float score_scale;
-  FastDiv by_page;
+  bool wide;  // rows of q and out start on 16 bytes
+  uint32_t group, blocks, vheads;  // query heads of a cache head, in blocks of 16; blocks of all heads
+  uint32_t ranges;                 // 0: a workgroup for each request
+  uint32_t start_words;            // LDS words of the requests' starts, a multiple of 4
+  uint32_t part_words;             // workspace words of a partial answer, a multiple of 4
+  uint32_t part_offset;            // and of the first one
+  FastDiv by_page, by_dim;
   uint32_t* status;
 };
 
 hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s);
 hipError_t launch_kv_append(const AppendArgs& a, uint32_t dtype, uint32_t kv_dtype, bool neighbours, uint32_t vec,
                             hipStream_t s);
-hipError_t launch_kv_attend(const AttendArgs& a, uint32_t dtype, uint32_t kv_dtype, hipStream_t s);
+hipError_t launch_attend_f32(const AttendArgs& a, hipStream_t s);
+hipError_t launch_attend_bf16(const AttendArgs& a, hipStream_t s);
+hipError_t launch_attend_f16(const AttendArgs& a, hipStream_t s);
+hipError_t launch_attend_e4m3_bf16(const AttendArgs& a, hipStream_t s);
+hipError_t launch_attend_e4m3_f16(const AttendArgs& a, hipStream_t s);
 
 }  // namespace llmhip

@@ -1,0 +1,327 @@
+// The tile products of the key-value cache's attention (kv_attend.h): how one
+// wave loads a tile of tokens and multiplies it on the matrix cores.
+//
+// Both products keep every operand where the loads and the first product put
+// it, so nothing moves between lanes. Lane = 16 g + c.
+//   S = K Q^T: row = token, column = query head. An MFMA's A operand has row
+//     c in this lane, its result columns c and rows 4 g + i. Which token a
+//     row stands for is free: row 4 x + i of the a-th product is token
+//     kGroup x + 4 a + i of the tile, so the results in lane (g, c) are
+//     query head c's scores of tokens kGroup g .. kGroup g + kGroup - 1.
+//   O = P V: row = query head, column = value. These same registers are the
+//     A operand (row c, tokens of group g), and a lane's B operand is column
+//     c of the same tokens: it loads kVec neighbouring values of each of its
+//     group's tokens, 16 lanes a row, and the j-th product takes the j-th
+//     value of each. Result columns are values c kVec + j.
+// The dot products' order of d is free too: the chunk that a lane of K
+// loads is the chunk that the same lane of Q loads.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "kv_types.h"
+
+namespace llmhip {
+
+using f32x4 = float __attribute__((ext_vector_type(4)));
+using u32x2 = uint32_t __attribute__((ext_vector_type(2)));
+using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
+using bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
+using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
+using f16x2 = _Float16 __attribute__((ext_vector_type(2)));
+using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
+
+template <class T, class F>
+__device__ __forceinline__ T bits_as(F x) {
+  static_assert(sizeof(T) == sizeof(F), "sizes differ");
+  return __builtin_bit_cast(T, x);
+}
+
+template <int BYTES>
+struct RawOf;
+template <>
+struct RawOf<4> { using type = uint32_t; };
+template <>
+struct RawOf<8> { using type = u32x2; };
+template <>
+struct RawOf<16> { using type = u32x4; };
+
+template <class T>
+__device__ __forceinline__ T load_raw(const char* p) {
+  return *reinterpret_cast<const T*>(p);
+}
+
+// The 16-bit types' products, 32 deep.
+__device__ __forceinline__ f32x4 mfma(BF16, u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bits_as<bf16x8>(a), bits_as<bf16x8>(b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma(F16, u32x4 a, u32x4 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(bits_as<f16x8>(a), bits_as<f16x8>(b), c, 0, 0, 0);
+}
+__device__ __forceinline__ uint32_t pack2(BF16, float x, float y) {
+  const bf16x2 v = {(__bf16)x, (__bf16)y};
+  return bits_as<uint32_t>(v);
+}
+__device__ __forceinline__ uint32_t pack2(F16, float x, float y) {
+  const f16x2 v = {(_Float16)x, (_Float16)y};
+  return bits_as<uint32_t>(v);
+}
+__device__ __forceinline__ void unpack2(BF16, uint32_t v, float& x, float& y) {
+  x = __uint_as_float(v << 16);
+  y = __uint_as_float(v & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack2(F16, uint32_t v, float& x, float& y) {
+  const f16x2 h = bits_as<f16x2>(v);
+  x = (float)h[0];
+  y = (float)h[1];
+}
+// Two E4M3 values of a word as 16-bit values, exactly.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t widen2(BF16, uint32_t x) {
+  return bits_as<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, HIGH));
+}
+template <bool HIGH>
+__device__ __forceinline__ uint32_t widen2(F16, uint32_t x) {
+  return bits_as<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, HIGH));
+}
+
+// Queries of a 16-bit type over a cache of that type or E4M3. DIM: head_dim
+// rounded up to 64, 128 or 256; FULL: it is head_dim.
+template <class Q_, class KV_, int DIM, bool FULL>
+struct Engine16 {
+  using Q = Q_;
+  using KV = KV_;
+  static constexpr int kElem = sizeof(typename KV::Raw);
+  static constexpr int kGroup = 8, kTile = 32, kProducts = 2;
+  static constexpr int kSteps = DIM / 32;
+  static constexpr int kVec = DIM == 64 ? 4 : 8, kPanels = DIM / (16 * kVec);
+  using KRaw = typename RawOf<8 * kElem>::type;
+  using VRaw = typename RawOf<kVec * kElem>::type;
+
+  u32x4 q[kSteps];
+  KRaw k[kProducts][kSteps];
+  VRaw v[kGroup][kPanels];
+  f32x4 o[kPanels][kVec];
+
+  // Byte offset of this lane's chunk of step s in a row, and whether the row
+  // has one (a lane without reads the row's start and drops it).
+  __device__ __forceinline__ static bool chunk(uint32_t s, uint32_t g, uint32_t dim, uint32_t& d) {
+    d = s * 32u + g * 8u;
+    if (FULL || d < dim) return true;
+    d = 0u;
+    return false;
+  }
+
+  __device__ __forceinline__ void load_q(const typename Q::Raw* row, uint32_t g, uint32_t dim, bool live, bool wide) {
+#pragma unroll
+    for (uint32_t s = 0; s < kSteps; ++s) {
+      uint32_t d;
+      const bool has = chunk(s, g, dim, d) && live;
+      u32x4 x = {0u, 0u, 0u, 0u};
+      if (has) {
+        if (wide) {
+          x = *reinterpret_cast<const u32x4*>(row + d);
+        } else {
+          const uint16_t* p = reinterpret_cast<const uint16_t*>(row + d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+        }
+      }
+      q[s] = x;
+    }
+  }
+
+  __device__ __forceinline__ void load_k(int a, const char* row, uint32_t g, uint32_t dim) {
+#pragma unroll
+    for (uint32_t s = 0; s < kSteps; ++s) {
+      uint32_t d;
+      chunk(s, g, dim, d);
+      k[a][s] = load_raw<KRaw>(row + d * kElem);
+    }
+  }
+
+  __device__ __forceinline__ void load_v(int i, const char* row, uint32_t c, uint32_t dim) {
+#pragma unroll
+    for (uint32_t p = 0; p < kPanels; ++p) {
+      const uint32_t d = (p * 16u + c) * kVec;
+      v[i][p] = load_raw<VRaw>(row + (FULL || d < dim ? d : 0u) * kElem);
+    }
+  }
+  __device__ __forceinline__ void drop_v(int i) {
+#pragma unroll
+    for (int p = 0; p < kPanels; ++p) v[i][p] = VRaw(0u);
+  }
+
+  // Scores of the lane's tokens.
+  __device__ __forceinline__ void scores(float* s, uint32_t g, uint32_t dim) const {
+#pragma unroll
+    for (int a = 0; a < kProducts; ++a) {
+      f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (uint32_t t = 0; t < kSteps; ++t) {
+        u32x4 y;
+        if constexpr (kElem == 1) {
+          y[0] = widen2<false>(Q(), k[a][t][0]);
+          y[1] = widen2<true>(Q(), k[a][t][0]);
+          y[2] = widen2<false>(Q(), k[a][t][1]);
+          y[3] = widen2<true>(Q(), k[a][t][1]);
+        } else {
+          y = k[a][t];
+        }
+        if (!FULL) {
+          uint32_t d;
+          const uint32_t keep = chunk(t, g, dim, d) ? ~0u : 0u;
+          y &= keep;
+        }
+        x = mfma(Q(), y, q[t], x);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[4 * a + i] = x[i];
+    }
+  }
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int p = 0; p < kPanels; ++p)
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) o[p][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  // Word w (values 2 w and 2 w + 1) of token i's values in panel p.
+  __device__ __forceinline__ uint32_t word(int i, int p, int w) const {
+    if constexpr (kElem == 1) {
+      uint32_t x;
+      if constexpr (kVec == 4) x = v[i][p];
+      else x = v[i][p][w >> 1];
+      return w & 1 ? widen2<true>(Q(), x) : widen2<false>(Q(), x);
+    } else {
+      return v[i][p][w];
+    }
+  }
+
+  // O += P V. A numerator is held as the sum of two 16-bit values, the
+  // second what the first one's rounding lost: the matrix cores have the time
+  // (24 products for 16 KiB of cache), and 16 bits of it are kept, not 8.
+  __device__ __forceinline__ void accumulate(const float* s) {
+    u32x4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      hi[i] = pack2(Q(), s[2 * i], s[2 * i + 1]);
+      float x, y;
+      unpack2(Q(), hi[i], x, y);
+      lo[i] = pack2(Q(), s[2 * i] - x, s[2 * i + 1] - y);
+    }
+#pragma unroll
+    for (int p = 0; p < kPanels; ++p) {
+#pragma unroll
+      for (int w = 0; w < kVec / 2; ++w) {
+        u32x4 even, odd;  // values 2 w and 2 w + 1 of the eight tokens
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x = word(2 * i, p, w), y = word(2 * i + 1, p, w);
+          even[i] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+          odd[i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+        }
+        o[p][2 * w] = mfma(Q(), lo, even, o[p][2 * w]);
+        o[p][2 * w + 1] = mfma(Q(), lo, odd, o[p][2 * w + 1]);
+        o[p][2 * w] = mfma(Q(), hi, even, o[p][2 * w]);
+        o[p][2 * w + 1] = mfma(Q(), hi, odd, o[p][2 * w + 1]);
+      }
+    }
+  }
+};
+
+// Queries and cache in binary32: the products are 4 deep, one token of each
+// group and one value of each chunk at a time.
+template <int DIM, bool FULL>
+struct Engine32 {
+  using Q = F32;
+  using KV = F32;
+  static constexpr int kElem = 4;
+  static constexpr int kGroup = 4, kTile = 16, kProducts = 1;
+  static constexpr int kSteps = DIM / 16;
+  static constexpr int kVec = 4, kPanels = DIM / 64;
+
+  f32x4 q[kSteps];
+  f32x4 k[kProducts][kSteps];
+  f32x4 v[kGroup][kPanels];
+  f32x4 o[kPanels][kVec];
+
+  __device__ __forceinline__ static bool chunk(uint32_t s, uint32_t g, uint32_t dim, uint32_t& d) {
+    d = s * 16u + g * 4u;
+    if (FULL || d < dim) return true;
+    d = 0u;
+    return false;
+  }
+
+  __device__ __forceinline__ void load_q(const float* row, uint32_t g, uint32_t dim, bool live, bool wide) {
+#pragma unroll
+    for (uint32_t s = 0; s < kSteps; ++s) {
+      uint32_t d;
+      const bool has = chunk(s, g, dim, d) && live;
+      f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (has) {
+        if (wide) {
+          x = *reinterpret_cast<const f32x4*>(row + d);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = row[d + i];
+        }
+      }
+      q[s] = x;
+    }
+  }
+
+  __device__ __forceinline__ void load_k(int a, const char* row, uint32_t g, uint32_t dim) {
+#pragma unroll
+    for (uint32_t s = 0; s < kSteps; ++s) {
+      uint32_t d;
+      chunk(s, g, dim, d);
+      k[a][s] = load_raw<f32x4>(row + d * kElem);
+    }
+  }
+
+  __device__ __forceinline__ void load_v(int i, const char* row, uint32_t c, uint32_t dim) {
+#pragma unroll
+    for (uint32_t p = 0; p < kPanels; ++p) {
+      const uint32_t d = (p * 16u + c) * kVec;
+      v[i][p] = load_raw<f32x4>(row + (FULL || d < dim ? d : 0u) * kElem);
+    }
+  }
+  __device__ __forceinline__ void drop_v(int i) {
+#pragma unroll
+    for (int p = 0; p < kPanels; ++p) v[i][p] = f32x4(0.0f);
+  }
+
+  __device__ __forceinline__ void scores(float* s, uint32_t g, uint32_t dim) const {
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (uint32_t t = 0; t < kSteps; ++t) {
+      uint32_t d;
+      const bool has = chunk(t, g, dim, d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x = __builtin_amdgcn_mfma_f32_16x16x4f32(has ? k[0][t][j] : 0.0f, q[t][j], x, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = x[i];
+  }
+
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int p = 0; p < kPanels; ++p)
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) o[p][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  __device__ __forceinline__ void accumulate(const float* s) {
+#pragma unroll
+    for (int i = 0; i < kGroup; ++i)
+#pragma unroll
+      for (int p = 0; p < kPanels; ++p)
+#pragma unroll
+        for (int j = 0; j < kVec; ++j)
+          o[p][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[i], v[i][p][j], o[p][j], 0, 0, 0);
+  }
+};
+
+}  // namespace llmhip
