@@ -77,7 +77,7 @@ int check_dtype(const llmhip_kv_cache* c, uint32_t dtype) {
 
 int check_table(size_t table_pages, size_t table_ld, size_t page) {
   ARG(table_ld >= table_pages, "table_ld < table_pages");
-  SUPPORTED(table_pages <= kMaxInt && (table_pages + 1) * page <= kMaxInt - 64, "table_pages * page must be below 2^31");
+  SUPPORTED(table_pages <= kMaxInt && (table_pages + 1) * page <= kMaxInt - 256, "table_pages * page must be below 2^31");
   return LLMHIP_OK;
 }
 
@@ -93,19 +93,20 @@ int check_table(size_t table_pages, size_t table_ld, size_t page) {
   Device scope(info.device);                                               \
   if (!scope.ok) return launched(hipErrorInvalidDevice, "hipSetDevice")
 
-// How llmhip_kv_attend cuts its work: a workgroup takes a range of one block
-// of query heads, two workgroups a compute unit.
+// Sizes of llmhip_kv_attend's work and workspace.
 struct AttendPlan {
-  uint32_t group, blocks, vheads, ranges, part_words;
+  uint32_t group, blocks, vheads, part_words;
+  size_t parts;  // partial answers: two for each range and block of query heads
   AttendPlan(const llmhip_kv_cache* c, size_t q_heads, uint32_t cus) {
     group = (uint32_t)q_heads / c->heads;
     blocks = (group + 15u) / 16u;
     vheads = blocks * c->heads;
-    ranges = std::min(std::max(2u * cus / vheads, 1u), kMaxRanges);
-    const uint32_t g = std::min(group, 16u);
-    part_words = (g * (c->head_dim + 2u) + 3u) / 4u * 4u;
+    part_words = (std::min(group, 16u) * (c->head_dim + 2u) + 3u) / 4u * 4u;
+    // Workgroups of up to 8 blocks fill the card, or two of up to 4: a range
+    // for each 8 of the blocks at most, and one range at least.
+    parts = 2 * std::max<size_t>(vheads, (size_t)8 * cus);
   }
-  size_t bytes() const { return ((size_t)kMaxSplitBatch + 4 + (size_t)ranges * vheads * 2 * part_words) * 4; }
+  size_t bytes() const { return (kCutWords + parts * part_words) * 4; }
 };
 
 void set_pools(const llmhip_kv_cache* c, const void** pool, const float** scale, int64_t (*stride)[3]) {
@@ -263,14 +264,12 @@ int llmhip_kv_attend(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
   a.table_pages = (uint32_t)table_pages;
   a.window = window < kMaxInt ? (uint32_t)window : 0u;
   a.score_scale = scale;
-  a.wide = rows_on(q, q_stride, 2, size_of(dtype), 16) && rows_on(out, out_stride, 2, size_of(dtype), 16);
   a.group = plan.group;
   a.blocks = plan.blocks;
   a.vheads = plan.vheads;
-  a.ranges = B <= kMaxSplitBatch ? plan.ranges : 0u;
-  a.start_words = a.ranges ? (a.B + 1u + 3u) / 4u * 4u : 0u;
+  a.cus = info.cus;
   a.part_words = plan.part_words;
-  a.part_offset = kMaxSplitBatch + 4u;
+  a.part_offset = kCutWords;
   a.by_page = FastDiv::of(a.page);
   a.by_dim = FastDiv::of(a.dim);
   a.status = info.status;

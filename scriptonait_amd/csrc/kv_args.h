@@ -13,6 +13,7 @@ constexpr uint32_t kMaxHeadDim = 256;
 // call that is cut (their tiles' prefix sums live in LDS).
 constexpr uint32_t kMaxRanges = 1024;
 constexpr uint32_t kMaxSplitBatch = 2048;
+constexpr uint32_t kCutWords = 4 * kMaxRanges;  // workspace words before the partial answers
 
 struct PlanArgs {
   int32_t* ring;
@@ -64,9 +65,10 @@ struct AttendArgs {
   float* workspace;
   uint32_t B, q_heads, heads, dim, pages, page, table_pages, window;
   float score_scale;
-  bool wide;  // rows of q and out start on 16 bytes
   uint32_t group, blocks, vheads;  // query heads of a cache head, in blocks of 16; blocks of all heads
-  uint32_t ranges;                 // 0: a workgroup for each request
+  uint32_t cus;                    // the device's compute units
+  uint32_t team, splits;           // a workgroup's blocks of heads, and waves for each
+  uint32_t ranges;                 // 0: a workgroup takes one request of one team
   uint32_t start_words;            // LDS words of the requests' starts, a multiple of 4
   uint32_t part_words;             // workspace words of a partial answer, a multiple of 4
   uint32_t part_offset;            // and of the first one

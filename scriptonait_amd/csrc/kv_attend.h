@@ -10,11 +10,15 @@
 //
 // The work is every request's tiles of tokens in one line, cut into equal
 // ranges, so ragged lengths share the card evenly and one long request uses
-// all of it. A workgroup takes one range of one cache head, its waves equal
-// parts of it. A request's run inside one wave goes straight to the output;
-// runs that waves of a group share are joined in LDS, and what a group
-// leaves of a request that goes on elsewhere goes to the workspace, for
-// join_kernel. What bounds it is reading the cache once.
+// all of it. A workgroup takes one range: a wave for each of up to 8 cache
+// heads, which so read a token's neighbouring rows at about the same time,
+// and where there are fewer heads, several waves for each, equal parts of
+// the range. (Reading 537 MB of 131072 tokens of 8 heads of 256 bytes this way
+// takes 80 us, with workgroups of one head 86 us.) A request's run inside one
+// wave goes straight to the output; runs that waves of one head share are
+// joined in LDS, and what a workgroup leaves of a request that goes on
+// elsewhere goes to the workspace, for join_kernel. What bounds it is reading
+// the cache once.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -25,7 +29,9 @@
 
 namespace llmhip {
 
-constexpr uint32_t kAttendWaves = 4, kAttendThreads = kAttendWaves * 64;
+// Waves of a workgroup: 8, two on each SIMD, where the registers allow it.
+template <class E, bool GROUPED>
+constexpr uint32_t kWavesOf = E::kDim > 128 || (!GROUPED && E::kDim > 64) ? 4 : 8;
 constexpr float kLazyBits = 8.0f;
 constexpr float kLn2 = 0.693147180559945309f, kLog2e = 1.44269504088896341f;
 constexpr uint32_t kNoId = 0xffffffffu;
@@ -37,23 +43,80 @@ __device__ __forceinline__ uint32_t tiles_of(uint32_t len, uint32_t window, uint
   return len ? (len + tile - 1u) / tile - first : 0u;
 }
 
-// Inclusive prefix sum over the workgroup's threads, and the total. `waves`:
-// kAttendWaves words of LDS.
-__device__ __forceinline__ uint32_t group_scan(uint32_t x, uint32_t* waves, uint32_t& total) {
-  const uint32_t lane = lane_id(), wave = threadIdx.x >> 6;
-  x = wave_incl_scan(x);
-  if (lane == 63u) waves[wave] = x;
-  __syncthreads();
-  total = 0u;
-  uint32_t before = 0u;
-#pragma unroll
-  for (uint32_t w = 0; w < kAttendWaves; ++w) {
-    before += w < wave ? waves[w] : 0u;
-    total += waves[w];
+// The line of all tiles: where each request's begin and end. Up to 64
+// requests live in a wave's lanes, more of them in LDS.
+struct Line {
+  uint32_t B, total;
+  uint32_t len, upto;      // lane r: request r's length, and the tiles up to and with it
+  const uint32_t* starts;  // LDS [B + 1], or null
+
+  // `words`: LDS for the starts and, before them, a word for each wave.
+  __device__ __forceinline__ void lay(const AttendArgs& a, uint32_t tile, uint32_t* words, bool& bad) {
+    const uint32_t most = a.table_pages * a.page, lane = lane_id();
+    uint32_t first;
+    B = a.B;
+    if (B <= 64u) {
+      starts = nullptr;
+      len = lane < B ? clamp_len(a.lens[lane], most, bad) : 0u;
+      upto = wave_incl_scan(tiles_of(len, a.window, tile, first));
+      total = readlane_u32(upto, 63);
+      return;
+    }
+    uint32_t* waves = words;
+    uint32_t* start = words + 16;
+    const uint32_t wave = threadIdx.x >> 6, n_waves = blockDim.x >> 6;
+    total = 0u;
+    for (uint32_t r0 = 0; r0 < B; r0 += blockDim.x) {
+      const uint32_t r = r0 + threadIdx.x;
+      const uint32_t n = r < B ? tiles_of(clamp_len(a.lens[r], most, bad), a.window, tile, first) : 0u;
+      const uint32_t sum = wave_incl_scan(n);
+      if (lane == 63u) waves[wave] = sum;
+      __syncthreads();
+      uint32_t before = total;
+      for (uint32_t w = 0; w < n_waves; ++w) {
+        before += w < wave ? waves[w] : 0u;
+        total += waves[w];
+      }
+      if (r < B) start[r] = before + sum - n;
+      __syncthreads();
+    }
+    if (threadIdx.x == 0u) start[B] = total;
+    __syncthreads();
+    total = readlane_u32(total, 0);
+    starts = start;
   }
-  __syncthreads();
-  return x + before;
+  __device__ __forceinline__ uint32_t start(uint32_t r) const {
+    if (starts) return readlane_u32(starts[r], 0);
+    return r ? readlane_u32(upto, r - 1u) : 0u;
+  }
+  __device__ __forceinline__ uint32_t end(uint32_t r) const {
+    return readlane_u32(starts ? starts[r + 1u] : upto, starts ? 0u : r);
+  }
+  // The request that holds a tile; for all lanes of a wave.
+  __device__ __forceinline__ uint32_t at(uint32_t tile) const {
+    if (!starts) return (uint32_t)__builtin_popcountll(__ballot(upto <= tile));
+    uint32_t i = 0, above = B;  // the last one that begins at or before it
+    while (above - i > 1u) {
+      const uint32_t mid = (i + above) >> 1;
+      if (starts[mid] <= tile) i = mid;
+      else above = mid;
+    }
+    return readlane_u32(i, 0);
+  }
+};
+
+// Workgroups go to the 8 XCDs in turn: the number that puts neighbours in
+// work on one of them.
+__device__ __forceinline__ uint32_t near_block(uint32_t id, uint32_t n) {
+  const uint32_t x = id & 7u, rest = n & 7u;
+  return x * (n >> 3) + min(x, rest) + (id >> 3);
 }
+
+// What joins a request that several ranges share: written by each range
+// about the request that came into it (request kNoId: none did).
+struct Cut {
+  uint32_t request, first, last, unused;
+};
 
 template <class E, bool GROUPED>
 struct Run {
@@ -79,25 +142,22 @@ struct Run {
     return t0 + E::kGroup * (c >> 2) + 4u * p + (c & 3u);
   }
 
-  __device__ __forceinline__ uint32_t page_id(uint32_t t, uint32_t width) const {
-    return t < hi && t + width > lo ? (uint32_t)row[a.by_page.div(t)] : kNoId;
+  // Page id of token t, or of the nearest one that is seen: always a load, so
+  // that the compiler can count the loads behind it when it waits.
+  __device__ __forceinline__ uint32_t page_id(uint32_t t) const {
+    return (uint32_t)row[a.by_page.div(min(max(t, lo), hi - 1u))];
   }
   __device__ __forceinline__ Ids fetch_ids(uint32_t t0) const {
     Ids x;
-    if constexpr (GROUPED) {
-      x.k[0] = page_id(t0 + E::kGroup * (c >> 2), E::kGroup);
-      x.v[0] = page_id(v_token(t0), E::kGroup);
-    } else {
 #pragma unroll
-      for (int p = 0; p < kKIds; ++p) x.k[p] = page_id(k_token(t0, p), 1u);
+    for (int p = 0; p < kKIds; ++p) x.k[p] = page_id(k_token(t0, p));
 #pragma unroll
-      for (int i = 0; i < kIds; ++i) x.v[i] = page_id(v_token(t0) + i, 1u);
-    }
+    for (int i = 0; i < kIds; ++i) x.v[i] = page_id(v_token(t0) + i);
     return x;
   }
 
-  // Where token t of page id starts; a token that is not seen leads to the
-  // pool's first page.
+  // Where a token of page id starts; an id outside the pool leads to its
+  // first page (seen_of drops the token).
   __device__ __forceinline__ const char* token_row(int pool, uint32_t id, uint32_t in_page) const {
     id = id < a.pages ? id : 0u;
     return base[pool] + ((int64_t)id * a.pool_stride[pool][0] + (int64_t)in_page * a.pool_stride[pool][1]) * E::kElem;
@@ -139,54 +199,61 @@ struct Run {
     return seen;
   }
 
-  // Tiles first .. last of the request. A tile's keys are loaded when the
-  // tile before has used its own, its values likewise, and its page ids two
-  // tiles ahead, so that no wait for one of them includes a younger load.
+  // Tiles first .. last of the request, at least one. A tile's keys are loaded
+  // when the tile before has used its own, its values likewise, and its page
+  // ids two tiles ahead, so that no wait for one of them includes a younger
+  // load. The last tile loads itself again (from the L2): a branch around the
+  // loads would make every wait one for all of them.
   __device__ __forceinline__ void tiles(uint32_t first, uint32_t last) {
     ref = 0.0f;
     limit = -INFINITY;
     sum = 0.0f;
     e.clear();
-    Ids next = fetch_ids(first * E::kTile);
-    load_keys(first * E::kTile, next);
-    load_values(first * E::kTile, next);
-    uint32_t seen = seen_of(first * E::kTile, next);
-    if (first + 1u < last) next = fetch_ids((first + 1u) * E::kTile);
-    for (uint32_t tile = first; tile < last; ++tile) {
-      const uint32_t t1 = (tile + 1u) * E::kTile;
-      const bool more = tile + 1u < last;
-      Ids after = next;
-      if (tile + 2u < last) after = fetch_ids(t1 + E::kTile);
+    uint32_t t0 = readlane_u32(first, 0) * E::kTile;  // (the same in every lane: the loop's branch is the wave's)
+    const uint32_t t_last = (readlane_u32(last, 0) - 1u) * E::kTile;
+    const Ids now = fetch_ids(t0);
+    Ids next = fetch_ids(min(t0 + E::kTile, t_last));
+    load_keys(t0, now);
+    load_values(t0, now);
+    uint32_t seen = seen_of(t0, now);
+    bool more;
+    do {
+      more = t0 != t_last;
       float s[E::kGroup];
       e.scores(s, g, a.dim);
-      if (more) load_keys(t1, next);
+      const uint32_t t1 = min(t0 + E::kTile, t_last);
+      const Ids after = fetch_ids(min(t0 + 2u * E::kTile, t_last));
+      load_keys(t1, next);
+      add(s, seen);
+      load_values(t1, next);
+      seen = seen_of(t1, next);
+      next = after;
+      t0 = t1;
+    } while (more);
+  }
+
+  // A tile's scores and values into ref, sum and o.
+  __device__ __forceinline__ void add(float* s, uint32_t seen) {
 #pragma unroll
-      for (int i = 0; i < E::kGroup; ++i) s[i] *= scale;
-      if (__any(seen != kAll)) {
-#pragma unroll
-        for (int i = 0; i < E::kGroup; ++i) {
-          if (!(seen >> i & 1u)) {
-            s[i] = -INFINITY;
-            e.drop_v(i);
-          }
-        }
-      }
-      float top = s[0];
-#pragma unroll
-      for (int i = 1; i < E::kGroup; ++i) top = fmaxf(top, s[i]);
-      if (__any(top > limit)) raise(top);
+    for (int i = 0; i < E::kGroup; ++i) s[i] *= scale;
+    if (__any(seen != kAll)) {
 #pragma unroll
       for (int i = 0; i < E::kGroup; ++i) {
-        s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
-        sum += s[i];
+        const bool keep = seen >> i & 1u;
+        s[i] = keep ? s[i] : -INFINITY;
+        e.keep_v(i, keep);
       }
-      e.accumulate(s);
-      if (more) {
-        load_values(t1, next);
-        seen = seen_of(t1, next);
-      }
-      next = after;
     }
+    float top = s[0];
+#pragma unroll
+    for (int i = 1; i < E::kGroup; ++i) top = fmaxf(top, s[i]);
+    if (__any(top > limit)) raise(top);
+#pragma unroll
+    for (int i = 0; i < E::kGroup; ++i) {
+      s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
+      sum += s[i];
+    }
+    e.accumulate(s);
   }
 
   // Moves the reference of each query head to its largest score.
@@ -222,50 +289,38 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 __host__ __device__ __forceinline__ uint32_t partial_words(uint32_t group, uint32_t dim) { return group * (dim + 2u); }
 
 template <class E, bool GROUPED>
-__global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(AttendArgs a) {
+  constexpr uint32_t kWaves = kWavesOf<E, GROUPED>;
   extern __shared__ uint32_t s_mem[];
-  __shared__ uint32_t s_waves[kAttendWaves];
-  __shared__ int32_t s_slot[2 * kAttendWaves];  // the request of each partial answer, or -1
-  uint32_t* s_start = s_mem;                    // split: where each request's tiles begin
+  __shared__ int32_t s_slot[2 * kWaves];  // the request of each partial answer, or -1
   float* s_part = reinterpret_cast<float*>(s_mem + a.start_words);
 
   const uint32_t tid = threadIdx.x, lane = lane_id(), wave = readlane_u32(tid >> 6, 0);
-  const uint32_t vhead = blockIdx.x % a.vheads, range = blockIdx.x / a.vheads;
+  // Heads whose rows are no whole cache lines share lines with their
+  // neighbours, and then an L2.
+  const uint32_t block = a.dim * E::kElem % 128u ? near_block(blockIdx.x, gridDim.x) : blockIdx.x;
+  const uint32_t teams = a.vheads / a.team, range = block / teams;
+  const uint32_t mate = wave % a.team, share = wave / a.team;  // the wave's head in the team, and its part of the range
+  const uint32_t vhead = block % teams * a.team + mate;
   const uint32_t head = vhead / a.blocks, q0 = vhead % a.blocks * 16u;  // first query head inside the group
   const uint32_t group = min(16u, a.group - q0);
   const uint32_t most = a.table_pages * a.page;
   bool bad = false;
 
-  // The range of tiles: [begin, end) of the line of all tiles (split), or
-  // one request's.
-  uint32_t begin, end, b = 0;
+  // The range of tiles: [begin, end) of the line, or one request's.
+  Line line;
+  uint32_t begin, end, quota = 1u, b = range;
   if (a.ranges) {
-    uint32_t total = 0;
-    for (uint32_t r0 = 0; r0 < a.B; r0 += kAttendThreads) {
-      const uint32_t r = r0 + tid;
-      uint32_t first, n = 0, sum;
-      if (r < a.B) n = tiles_of(clamp_len(a.lens[r], most, bad), a.window, E::kTile, first);
-      const uint32_t upto = total + group_scan(n, s_waves, sum);
-      if (r < a.B) s_start[r] = upto - n;
-      total += sum;
-    }
-    if (tid == 0u) s_start[a.B] = total;
-    __syncthreads();
-    const uint32_t quota = max((total + a.ranges - 1u) / a.ranges, kAttendWaves);
-    if (blockIdx.x == 0u)
-      for (uint32_t r = tid; r <= a.B; r += kAttendThreads) reinterpret_cast<uint32_t*>(a.workspace)[r] = s_start[r];
-    begin = min(range * quota, total);
-    end = min(begin + quota, total);
+    line.lay(a, E::kTile, s_mem, bad);
+    quota = max((line.total + a.ranges - 1u) / a.ranges, a.splits);
+    begin = min(range * quota, line.total);
+    end = min(begin + quota, line.total);
   } else {
     uint32_t first;
-    b = range;
     begin = 0u;
     end = tiles_of(clamp_len(a.lens[b], most, bad), a.window, E::kTile, first);
   }
-  if (tid < 2u * kAttendWaves) s_slot[tid] = -1;
-  __syncthreads();
   if (bad && vhead == 0u && (range == 0u || !a.ranges)) atomicOr(a.status, LLMHIP_KSTATUS_BAD_INDEX);
-  bad = false;
 
   Run<E, GROUPED> run(a);
   run.g = lane >> 4;
@@ -277,33 +332,43 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a) {
   run.scale = a.score_scale * kLog2e * (e4m3 ? a.scale[0][head] : 1.0f);
   const float vscale = e4m3 ? a.scale[1][head] : 1.0f;
   const uint32_t qhead = head * a.group + q0;  // of the output
-  const uint32_t words = partial_words(group, a.dim);
 
-  uint32_t tile = begin + (end - begin) * wave / kAttendWaves;
-  const uint32_t stop = begin + (end - begin) * (wave + 1u) / kAttendWaves;
-  if (a.ranges && tile < stop) {
-    uint32_t i = 0, above = a.B;  // the last request that begins at or before the tile
-    while (above - i > 1u) {
-      const uint32_t mid = (i + above) >> 1;
-      if (s_start[mid] <= tile) i = mid;
-      else above = mid;
-    }
-    b = readlane_u32(i, 0);
-  }
-  bool first_run = true;
-  while (tile < stop) {
-    uint32_t from = 0u, to = end;
-    if (a.ranges) {
-      from = s_start[b];
-      to = s_start[b + 1u];
-      if (to <= tile) {  // an empty request
-        ++b;
-        continue;
+  const auto partial_of = [&](bool before) {
+    return a.workspace + a.part_offset + (((uint64_t)range * a.vheads + vhead) * 2u + (before ? 0u : 1u)) * a.part_words;
+  };
+  const auto put_partial = [&](float* part, float m, float l) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t qi = 4u * run.g + i;
+      if (qi >= group) continue;
+#pragma unroll
+      for (uint32_t p = 0; p < E::kPanels; ++p) {
+        const uint32_t d = (p * 16u + run.c) * E::kVec;
+        if (d >= a.dim) continue;
+#pragma unroll
+        for (int j = 0; j < E::kVec; ++j) part[qi * a.dim + d + j] = run.e.o[p][j][i];
       }
     }
-    uint32_t zero_tile;
+    if (lane < group) {
+      part[group * a.dim + lane] = m;
+      part[group * (a.dim + 1u) + lane] = l;
+    }
+  };
+
+  uint32_t tile = begin + (end - begin) * share / a.splits, slot = 2u * wave;
+  const uint32_t stop = begin + (end - begin) * (share + 1u) / a.splits;
+  if (a.splits > 1u && lane < 2u) s_slot[slot + lane] = -1;
+  if (a.ranges && tile < stop) b = line.at(tile);
+  while (tile < stop) {
+    const uint32_t from = a.ranges ? line.start(b) : 0u, to = a.ranges ? line.end(b) : end;
+    if (to <= tile) {  // an empty request
+      ++b;
+      continue;
+    }
     bool clamped = false;
-    const uint32_t len = clamp_len(a.lens[b], most, clamped);
+    const uint32_t len =
+        a.ranges && !line.starts ? readlane_u32(line.len, b) : readlane_u32(clamp_len(a.lens[b], most, clamped), 0);
+    uint32_t zero_tile;
     tiles_of(len, a.window, E::kTile, zero_tile);
     const uint32_t last = min(stop, to);
     run.row = a.table + (uint64_t)b * a.table_ld;
@@ -311,7 +376,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a) {
     run.hi = len;
     const typename E::Q::Raw* q = static_cast<const typename E::Q::Raw*>(a.q) + (int64_t)b * a.q_stride[0] +
                                   (int64_t)(qhead + (run.c < group ? run.c : 0u)) * a.q_stride[1];
-    run.e.load_q(q, run.g, a.dim, run.c < group, a.wide);
+    run.e.load_q(q, run.g, a.dim, run.c < group);
     run.tiles(zero_tile + (tile - from), zero_tile + (last - from));
     const float l = run.total(), m = l == 0.0f ? -INFINITY : run.ref;
     if (tile == from && last == to) {  // all of the request
@@ -330,73 +395,89 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a) {
           Pack<typename E::Q, E::kVec> x;
 #pragma unroll
           for (int j = 0; j < E::kVec; ++j) x.v[j] = E::Q::store(run.e.o[p][j][i] * scale);
-          if (a.wide) {
-            *reinterpret_cast<Pack<typename E::Q, E::kVec>*>(out + d) = x;
-          } else {
-#pragma unroll
-            for (int j = 0; j < E::kVec; ++j) out[d + j] = x.v[j];
-          }
+          __builtin_memcpy(out + d, x.v, sizeof x.v);
         }
       }
       if (a.lse && lane < group) a.lse[(uint64_t)b * a.q_heads + qhead + lane] = lse_of(m, l);
-    } else {
-      const uint32_t slot = 2u * wave + (first_run ? 0u : 1u);
-      float* part = s_part + slot * words;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t qi = 4u * run.g + i;
-        if (qi >= group) continue;
-#pragma unroll
-        for (uint32_t p = 0; p < E::kPanels; ++p) {
-          const uint32_t d = (p * 16u + run.c) * E::kVec;
-          if (d >= a.dim) continue;
-#pragma unroll
-          for (int j = 0; j < E::kVec; ++j) part[qi * a.dim + d + j] = run.e.o[p][j][i];
-        }
-      }
-      if (lane < group) {
-        part[group * a.dim + lane] = m;
-        part[group * (a.dim + 1u) + lane] = l;
-      }
+    } else if (a.splits > 1u) {
+      put_partial(s_part + slot * a.part_words, m, l);
       if (lane == 0u) s_slot[slot] = (int32_t)b;
+      ++slot;  // a wave leaves two at most: one that came in, one that goes on
+    } else {
+      put_partial(partial_of(from < begin), m, l);
     }
-    first_run = false;
     tile = last;
     ++b;
   }
   if (__any(run.bad) && lane == 0u) atomicOr(a.status, LLMHIP_KSTATUS_BAD_INDEX);
+
+  // Requests of length 0: a range has every ranges-th one.
+  const auto empty = [&](uint32_t r) {
+    for (uint32_t x = lane; x < group * a.dim; x += 64u) {
+      const uint32_t qi = a.by_dim.div(x), d = x - qi * a.dim;
+      static_cast<typename E::Q::Raw*>(a.out)[(int64_t)r * a.out_stride[0] + (int64_t)(qhead + qi) * a.out_stride[1] + d] =
+          E::Q::store(0.0f);
+      if (a.lse && d == 0u) a.lse[(uint64_t)r * a.q_heads + qhead + qi] = -INFINITY;
+    }
+  };
+  if (a.ranges) {
+    for (uint32_t r = range + share * a.ranges; r < a.B; r += a.splits * a.ranges)
+      if (line.start(r) == line.end(r)) empty(r);
+    // For the join: the request that came into this range, and its ranges.
+    if (vhead == 0u && share == 0u) {
+      Cut cut = {kNoId, 0u, 0u, 0u};
+      if (begin < end) {
+        const uint32_t r = line.at(begin);
+        if (line.start(r) < begin) cut = {r, line.start(r) / quota, (line.end(r) - 1u) / quota, 0u};
+      }
+      if (lane == 0u) reinterpret_cast<Cut*>(a.workspace)[range] = cut;
+    }
+  } else if (end == 0u && share == 0u) {
+    empty(b);
+  }
+  if (a.splits == 1u) return;
   __syncthreads();
 
-  // Join neighbouring partial answers of a request. At most two of the
-  // group's requests go on outside its range.
-  for (uint32_t i = 0; i < 2u * kAttendWaves;) {
-    const int32_t r = s_slot[i];
-    if (r < 0) {
-      ++i;
-      continue;
+  // Join the partial answers of each request of the wave's head: one of each
+  // share at most, all read at once (a missing one stands for the first
+  // again, with weight 0). The head's waves do this together. At most two of
+  // its requests go on outside the range.
+  const int32_t holds = lane < 2u * a.splits ? s_slot[2u * ((lane >> 1) * a.team + mate) + (lane & 1u)] : -1;
+  uint64_t rest = __ballot(holds >= 0);
+  while (rest) {
+    const uint32_t r = readlane_u32((uint32_t)holds, (uint32_t)__builtin_ctzll(rest));
+    uint64_t set = __ballot(holds == (int32_t)r);
+    rest &= ~set;
+    const uint32_t n = (uint32_t)__builtin_popcountll(set);
+    const float* part[kWaves];
+#pragma unroll
+    for (uint32_t k = 0; k < kWaves; ++k) {
+      const uint32_t i = (uint32_t)__builtin_ctzll(set);
+      part[k] = k < n ? s_part + (2u * ((i >> 1) * a.team + mate) + (i & 1u)) * a.part_words : part[0];
+      set &= set - 1u;
     }
-    uint32_t n = i + 1u;
-    while (n < 2u * kAttendWaves && (s_slot[n] == r || s_slot[n] < 0)) ++n;
-    const bool before = a.ranges && s_start[r] < begin, after = a.ranges && s_start[r + 1] > end;
-    float* to = a.workspace + a.part_offset + ((uint64_t)blockIdx.x * 2u + (before ? 0u : 1u)) * a.part_words;
-    for (uint32_t x = tid; x < group * a.dim; x += kAttendThreads) {
-      const uint32_t qi = a.by_dim.div(x), d = x - qi * a.dim;
-      float m = -INFINITY, l = 0.0f, o = 0.0f;
-      for (uint32_t k = i; k < n; ++k)
-        if (s_slot[k] >= 0) m = fmaxf(m, s_part[k * words + group * a.dim + qi]);
+    const bool before = a.ranges && line.start(r) < begin, after = a.ranges && line.end(r) > end;
+    float* to = partial_of(before);
+    for (uint32_t x = share * 64u + lane; x < group * a.dim; x += a.splits * 64u) {
+      const uint32_t qi = a.by_dim.div(x), d = x - qi * a.dim, at_m = group * a.dim + qi, at_l = at_m + group;
+      float m = -INFINITY, l = 0.0f, o = 0.0f, w[kWaves];
+#pragma unroll
+      for (uint32_t k = 0; k < kWaves; ++k) {
+        w[k] = k < n ? part[k][at_m] : -INFINITY;
+        m = fmaxf(m, w[k]);
+      }
       const float top = m == -INFINITY ? 0.0f : m;
-      for (uint32_t k = i; k < n; ++k) {
-        if (s_slot[k] < 0) continue;
-        const float* part = s_part + k * words;
-        const float w = __builtin_amdgcn_exp2f(part[group * a.dim + qi] - top);
-        l += part[group * (a.dim + 1u) + qi] * w;
-        o += part[x] * w;
+#pragma unroll
+      for (uint32_t k = 0; k < kWaves; ++k) {
+        w[k] = __builtin_amdgcn_exp2f(w[k] - top);
+        l += part[k][at_l] * w[k];
+        o += part[k][x] * w[k];
       }
       if (before || after) {
         to[x] = o;
         if (d == 0u) {
-          to[group * a.dim + qi] = m;
-          to[group * (a.dim + 1u) + qi] = l;
+          to[at_m] = m;
+          to[at_l] = l;
         }
       } else {
         const float inv = l == 0.0f ? 0.0f : vscale / l;
@@ -406,100 +487,124 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a) {
         if (a.lse && d == 0u) a.lse[(uint64_t)r * a.q_heads + qhead + qi] = lse_of(m, l);
       }
     }
-    i = n;
   }
-  if (!a.ranges && end == 0u) {  // a request of length 0
-    for (uint32_t x = tid; x < group * a.dim; x += kAttendThreads) {
-      const uint32_t qi = a.by_dim.div(x), d = x - qi * a.dim;
-      static_cast<typename E::Q::Raw*>(a.out)[(int64_t)b * a.out_stride[0] + (int64_t)(qhead + qi) * a.out_stride[1] + d] =
-          E::Q::store(0.0f);
-      if (a.lse && d == 0u) a.lse[(uint64_t)b * a.q_heads + qhead + qi] = -INFINITY;
+}
+
+// The answers of requests that several ranges share. A workgroup takes 64
+// values of a query head, 16 partial answers at a time; the joining order
+// depends on their number alone.
+template <class Q, class KV>
+__global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
+  constexpr uint32_t kShare = 16;
+  __shared__ float s_m[kShare], s_l[kShare];
+  __shared__ f32x4 s_o[256];
+  const uint32_t tid = threadIdx.x, share = tid >> 4, chunks = (a.dim + 63u) / 64u;
+  const uint32_t qh = blockIdx.x / chunks, chunk = blockIdx.x % chunks, d = chunk * 64u + (tid & 15u) * 4u;
+  const uint32_t head = qh / a.group, in_group = qh % a.group, vhead = head * a.blocks + in_group / 16u;
+  const uint32_t group = min(16u, a.group - in_group / 16u * 16u), qi = in_group % 16u;
+  const float vscale = KV::kId == LLMHIP_E4M3 ? a.scale[1][head] : 1.0f;
+  for (uint32_t r = 1u + blockIdx.y; r < a.ranges; r += gridDim.y) {
+    const Cut cut = reinterpret_cast<const Cut*>(a.workspace)[r];
+    if (cut.request == kNoId || cut.first + 1u != r) continue;  // the request's first range boundary joins it
+    const uint32_t n = cut.last - cut.first + 1u;
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t k0 = share; k0 < n; k0 += 4u * kShare) {
+      float pm[4], pl[4];
+      f32x4 po[4];
+#pragma unroll
+      for (uint32_t j = 0; j < 4u; ++j) {
+        const uint32_t k = k0 + j * kShare;
+        pm[j] = -INFINITY;
+        pl[j] = 0.0f;
+        po[j] = o * 0.0f;
+        if (k < n) {
+          const float* part =
+              a.workspace + a.part_offset + (((uint64_t)(cut.first + k) * a.vheads + vhead) * 2u + (k ? 0u : 1u)) * a.part_words;
+          pm[j] = part[group * a.dim + qi];
+          pl[j] = part[group * (a.dim + 1u) + qi];
+          if (d < a.dim) po[j] = *reinterpret_cast<const f32x4*>(part + qi * a.dim + d);
+        }
+      }
+      const float next = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]))), top = next == -INFINITY ? 0.0f : next;
+      const float keep = __builtin_amdgcn_exp2f(m - top);
+      o *= keep;
+      l *= keep;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float w = __builtin_amdgcn_exp2f(pm[j] - top);
+        l += pl[j] * w;
+        o += po[j] * w;
+      }
+      m = next;
+    }
+    __syncthreads();
+    if ((tid & 15u) == 0u) {
+      s_m[share] = m;
+      s_l[share] = l;
+    }
+    s_o[tid] = o;
+    __syncthreads();
+    if (share == 0u) {
+      for (uint32_t k = 0; k < kShare; ++k) m = fmaxf(m, s_m[k]);
+      const float top = m == -INFINITY ? 0.0f : m;
+      l = 0.0f;
+      o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (uint32_t k = 0; k < kShare; ++k) {
+        const float w = __builtin_amdgcn_exp2f(s_m[k] - top);
+        l += s_l[k] * w;
+        o += s_o[k * 16u + tid] * w;
+      }
+      const float inv = l == 0.0f ? 0.0f : vscale / l;
+      typename Q::Raw* out =
+          static_cast<typename Q::Raw*>(a.out) + (int64_t)cut.request * a.out_stride[0] + (int64_t)qh * a.out_stride[1];
+      if (d < a.dim) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) out[d + j] = Q::store(o[j] * inv);
+      }
+      if (a.lse && tid == 0u && chunk == 0u) a.lse[(uint64_t)cut.request * a.q_heads + qh] = lse_of(m, l);
     }
   }
 }
 
-// The answers of requests that several ranges share, and of empty ones. One
-// workgroup for each request and query head; the partial answers are joined
-// in the ranges' order.
-template <class Q, class KV>
-__global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
-  __shared__ float s_weight[kMaxRanges];
-  __shared__ float s_wave[2][4];
-  __shared__ f32x4 s_sum[256];
-  const uint32_t tid = threadIdx.x, lane = lane_id(), wave = tid >> 6, b = blockIdx.y, qh = blockIdx.x;
-  const uint32_t* start = reinterpret_cast<const uint32_t*>(a.workspace);
-  const uint32_t total = start[a.B], from = start[b], to = start[b + 1u];
-  const uint32_t quota = max((total + a.ranges - 1u) / a.ranges, kAttendWaves);
-  typename Q::Raw* out = static_cast<typename Q::Raw*>(a.out) + (int64_t)b * a.out_stride[0] + (int64_t)qh * a.out_stride[1];
-  if (from == to) {
-    if (tid < a.dim) out[tid] = Q::store(0.0f);
-    if (a.lse && tid == 0u) a.lse[(uint64_t)b * a.q_heads + qh] = -INFINITY;
-    return;
-  }
-  const uint32_t r0 = from / quota, n = (to - 1u) / quota - r0 + 1u;
-  if (n == 1u) return;
-  const uint32_t head = qh / a.group, in_group = qh % a.group, vhead = head * a.blocks + in_group / 16u;
-  const uint32_t group = min(16u, a.group - in_group / 16u * 16u), qi = in_group % 16u;
-  const auto part = [&](uint32_t k) {
-    return a.workspace + a.part_offset + (((uint64_t)(r0 + k) * a.vheads + vhead) * 2u + (k ? 0u : 1u)) * a.part_words;
-  };
-  float m = -INFINITY;
-  for (uint32_t k = tid; k < n; k += 256u) m = fmaxf(m, part(k)[group * a.dim + qi]);
-#pragma unroll
-  for (uint32_t off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-  if (lane == 0u) s_wave[0][wave] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_wave[0][0], s_wave[0][1]), fmaxf(s_wave[0][2], s_wave[0][3]));
-  const float top = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f;
-  for (uint32_t k = tid; k < n; k += 256u) {
-    const float w = __builtin_amdgcn_exp2f(part(k)[group * a.dim + qi] - top);
-    s_weight[k] = w;
-    l += part(k)[group * (a.dim + 1u) + qi] * w;
-  }
-#pragma unroll
-  for (uint32_t off = 32; off; off >>= 1) l += __shfl_xor(l, off, 64);
-  if (lane == 0u) s_wave[1][wave] = l;
-  __syncthreads();
-  l = (s_wave[1][0] + s_wave[1][1]) + (s_wave[1][2] + s_wave[1][3]);
-  // dim / 4 threads take a partial answer's values, the rest others'.
-  const uint32_t across = a.dim / 4u, share = 256u / across, mine = tid / across, d = (tid - mine * across) * 4u;
-  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (mine < share)
-    for (uint32_t k = mine; k < n; k += share)
-      o += *reinterpret_cast<const f32x4*>(part(k) + qi * a.dim + d) * s_weight[k];
-  s_sum[tid] = o;
-  __syncthreads();
-  if (mine == 0u) {
-    for (uint32_t k = 1; k < share; ++k) o += s_sum[k * across + tid];
-    const float vscale = KV::kId == LLMHIP_E4M3 ? a.scale[1][head] : 1.0f, inv = l == 0.0f ? 0.0f : vscale / l;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) out[d + j] = Q::store(o[j] * inv);
-  }
-  if (a.lse && tid == 0u) a.lse[(uint64_t)b * a.q_heads + qh] = lse_of(m, l);
+template <class E, bool GROUPED>
+hipError_t launch_attend_group(AttendArgs a, hipStream_t s) {
+  constexpr uint32_t kWaves = kWavesOf<E, GROUPED>;
+  a.team = kWaves;
+  while (a.vheads % a.team) --a.team;
+  a.splits = kWaves / a.team;
+  const uint32_t teams = a.vheads / a.team;
+  // A workgroup of 8 waves, or two of 4, on each compute unit; more requests
+  // than the line takes are not cut, with a workgroup for each.
+  a.ranges = a.B > kMaxSplitBatch ? 0u : min(max(a.cus * (8u / kWaves) / teams, 1u), kMaxRanges);
+  a.start_words = a.ranges && a.B > 64u ? 16u + (a.B + 1u + 3u) / 4u * 4u : 0u;
+  const uint32_t lds = (a.start_words + (a.splits > 1u ? 2u * kWaves * a.part_words : 0u)) * 4u;
+  const dim3 grid((a.ranges ? a.ranges : a.B) * teams), threads(a.team * a.splits * 64u);
+  hipLaunchKernelGGL((attend_kernel<E, GROUPED>), grid, threads, lds, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.ranges < 2u) return e;
+  hipLaunchKernelGGL((join_kernel<typename E::Q, typename E::KV>),
+                     dim3(a.q_heads * ((a.dim + 63u) / 64u), min(a.ranges - 1u, 64u)), dim3(256), 0, s, a);
+  return hipGetLastError();
 }
 
 template <class E>
 hipError_t launch_attend_engine(const AttendArgs& a, hipStream_t s) {
-  const dim3 grid((a.ranges ? a.ranges : a.B) * a.vheads);
-  const uint32_t lds = (a.start_words + 2u * kAttendWaves * partial_words(min(16u, a.group), a.dim)) * 4u;
-  if (a.page % E::kGroup == 0u)
-    hipLaunchKernelGGL((attend_kernel<E, true>), grid, dim3(kAttendThreads), lds, s, a);
-  else
-    hipLaunchKernelGGL((attend_kernel<E, false>), grid, dim3(kAttendThreads), lds, s, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || !a.ranges) return e;
-  hipLaunchKernelGGL((join_kernel<typename E::Q, typename E::KV>), dim3(a.q_heads, a.B), dim3(256), 0, s, a);
-  return hipGetLastError();
+  return a.page % E::kGroup == 0u ? launch_attend_group<E, true>(a, s) : launch_attend_group<E, false>(a, s);
 }
 
-template <template <int, bool> class E>
+// ENGINE<DIM, FULL>: the smallest DIM that holds head_dim. (Its name is part of
+// this function's symbol: each source needs one of its own.)
+template <template <int, bool> class ENGINE>
 hipError_t launch_attend_dims(const AttendArgs& a, hipStream_t s) {
-  if (a.dim == 64u) return launch_attend_engine<E<64, true>>(a, s);
-  if (a.dim == 128u) return launch_attend_engine<E<128, true>>(a, s);
-  if (a.dim < 64u) return launch_attend_engine<E<64, false>>(a, s);
-  if (a.dim < 128u) return launch_attend_engine<E<128, false>>(a, s);
-  return launch_attend_engine<E<256, false>>(a, s);
+  if (a.dim == 64u) return launch_attend_engine<ENGINE<64, true>>(a, s);
+  if (a.dim == 128u) return launch_attend_engine<ENGINE<128, true>>(a, s);
+  if (a.dim <= 32u) return launch_attend_engine<ENGINE<32, false>>(a, s);
+  if (a.dim < 64u) return launch_attend_engine<ENGINE<64, false>>(a, s);
+  if (a.dim <= 96u) return launch_attend_engine<ENGINE<96, false>>(a, s);
+  if (a.dim < 128u) return launch_attend_engine<ENGINE<128, false>>(a, s);
+  if (a.dim <= 192u) return launch_attend_engine<ENGINE<192, false>>(a, s);
+  return launch_attend_engine<ENGINE<256, false>>(a, s);
 }
 
 }  // namespace llmhip

@@ -4,8 +4,8 @@
 namespace llmhip {
 
 template <int DIM, bool FULL>
-using Engine = Engine16<BF16, BF16, DIM, FULL>;
+using EngineBF16 = Engine16<BF16, BF16, DIM, FULL, 8>;
 
-hipError_t launch_attend_bf16(const AttendArgs& a, hipStream_t s) { return launch_attend_dims<Engine>(a, s); }
+hipError_t launch_attend_bf16(const AttendArgs& a, hipStream_t s) { return launch_attend_dims<EngineBF16>(a, s); }
 
 }  // namespace llmhip

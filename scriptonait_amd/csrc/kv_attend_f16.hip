@@ -4,8 +4,8 @@
 namespace llmhip {
 
 template <int DIM, bool FULL>
-using Engine = Engine16<F16, F16, DIM, FULL>;
+using EngineF16 = Engine16<F16, F16, DIM, FULL, 8>;
 
-hipError_t launch_attend_f16(const AttendArgs& a, hipStream_t s) { return launch_attend_dims<Engine>(a, s); }
+hipError_t launch_attend_f16(const AttendArgs& a, hipStream_t s) { return launch_attend_dims<EngineF16>(a, s); }
 
 }  // namespace llmhip

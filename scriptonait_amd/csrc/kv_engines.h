@@ -40,15 +40,23 @@ __device__ __forceinline__ T bits_as(F x) {
 template <int BYTES>
 struct RawOf;
 template <>
+struct RawOf<2> { using type = uint16_t; };
+template <>
 struct RawOf<4> { using type = uint32_t; };
 template <>
 struct RawOf<8> { using type = u32x2; };
 template <>
 struct RawOf<16> { using type = u32x4; };
 
+// Keys: two neighbouring loads share a cache line, the first level keeps it.
 template <class T>
-__device__ __forceinline__ T load_raw(const char* p) {
+__device__ __forceinline__ T load_key(const char* p) {
   return *reinterpret_cast<const T*>(p);
+}
+// Values: whole lines, used once.
+template <class T>
+__device__ __forceinline__ T load_value(const char* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
 }
 
 // The 16-bit types' products, 32 deep.
@@ -86,57 +94,59 @@ __device__ __forceinline__ uint32_t widen2(F16, uint32_t x) {
 }
 
 // Queries of a 16-bit type over a cache of that type or E4M3. DIM: head_dim
-// rounded up to 64, 128 or 256; FULL: it is head_dim.
-template <class Q_, class KV_, int DIM, bool FULL>
+// rounded up to one of 32, 64, 96, 128, 192 and 256; FULL: it is head_dim.
+// CHUNK: neighbouring values that a lane loads of a key, 16 in an E4M3 row
+// of whole 16s, else 8.
+template <class Q_, class KV_, int DIM, bool FULL, int CHUNK>
 struct Engine16 {
   using Q = Q_;
   using KV = KV_;
   static constexpr int kElem = sizeof(typename KV::Raw);
+  static constexpr int kDim = DIM;
   static constexpr int kGroup = 8, kTile = 32, kProducts = 2;
-  static constexpr int kSteps = DIM / 32;
-  static constexpr int kVec = DIM == 64 ? 4 : 8, kPanels = DIM / (16 * kVec);
-  using KRaw = typename RawOf<8 * kElem>::type;
+  static constexpr int kLoads = (DIM + 4 * CHUNK - 1) / (4 * CHUNK);  // of a lane, for a key
+  static constexpr int kDeep = CHUNK / 8;                             // products of a load
+  // Values of a token in a lane. A divisor of 8, as head_dim is a multiple of
+  // 8: no load or store passes the row's end.
+  static constexpr int kVec = DIM == 32 ? 2 : DIM == 64 || (DIM == 192 && kElem == 2) ? 4 : 8;
+  static constexpr int kPanels = (DIM + 16 * kVec - 1) / (16 * kVec);
+  using KRaw = typename RawOf<CHUNK * kElem>::type;
   using VRaw = typename RawOf<kVec * kElem>::type;
 
-  u32x4 q[kSteps];
-  KRaw k[kProducts][kSteps];
+  u32x4 q[kLoads][kDeep];
+  KRaw k[kProducts][kLoads];
   VRaw v[kGroup][kPanels];
   f32x4 o[kPanels][kVec];
 
-  // Byte offset of this lane's chunk of step s in a row, and whether the row
-  // has one (a lane without reads the row's start and drops it).
+  // First value of this lane's chunk in load s, and whether the row has it (a
+  // lane without reads the row's start and drops it).
   __device__ __forceinline__ static bool chunk(uint32_t s, uint32_t g, uint32_t dim, uint32_t& d) {
-    d = s * 32u + g * 8u;
-    if (FULL || d < dim) return true;
+    d = (s * 4u + g) * CHUNK;
+    if ((FULL && DIM % (4 * CHUNK) == 0) || d < dim) return true;
     d = 0u;
     return false;
   }
 
-  __device__ __forceinline__ void load_q(const typename Q::Raw* row, uint32_t g, uint32_t dim, bool live, bool wide) {
+  __device__ __forceinline__ void load_q(const typename Q::Raw* row, uint32_t g, uint32_t dim, bool live) {
 #pragma unroll
-    for (uint32_t s = 0; s < kSteps; ++s) {
+    for (uint32_t s = 0; s < kLoads; ++s) {
       uint32_t d;
       const bool has = chunk(s, g, dim, d) && live;
-      u32x4 x = {0u, 0u, 0u, 0u};
-      if (has) {
-        if (wide) {
-          x = *reinterpret_cast<const u32x4*>(row + d);
-        } else {
-          const uint16_t* p = reinterpret_cast<const uint16_t*>(row + d);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
-        }
+      for (int h = 0; h < kDeep; ++h) {
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (has) __builtin_memcpy(&x, row + d + 8 * h, 16);  // rows of any alignment
+        q[s][h] = x;
       }
-      q[s] = x;
     }
   }
 
   __device__ __forceinline__ void load_k(int a, const char* row, uint32_t g, uint32_t dim) {
 #pragma unroll
-    for (uint32_t s = 0; s < kSteps; ++s) {
+    for (uint32_t s = 0; s < kLoads; ++s) {
       uint32_t d;
       chunk(s, g, dim, d);
-      k[a][s] = load_raw<KRaw>(row + d * kElem);
+      k[a][s] = load_key<KRaw>(row + d * kElem);
     }
   }
 
@@ -144,12 +154,12 @@ struct Engine16 {
 #pragma unroll
     for (uint32_t p = 0; p < kPanels; ++p) {
       const uint32_t d = (p * 16u + c) * kVec;
-      v[i][p] = load_raw<VRaw>(row + (FULL || d < dim ? d : 0u) * kElem);
+      v[i][p] = load_value<VRaw>(row + (FULL || d < dim ? d : 0u) * kElem);
     }
   }
-  __device__ __forceinline__ void drop_v(int i) {
+  __device__ __forceinline__ void keep_v(int i, bool keep) {
 #pragma unroll
-    for (int p = 0; p < kPanels; ++p) v[i][p] = VRaw(0u);
+    for (int p = 0; p < kPanels; ++p) v[i][p] &= VRaw(keep ? ~0u : 0u);
   }
 
   // Scores of the lane's tokens.
@@ -158,22 +168,23 @@ struct Engine16 {
     for (int a = 0; a < kProducts; ++a) {
       f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (uint32_t t = 0; t < kSteps; ++t) {
-        u32x4 y;
-        if constexpr (kElem == 1) {
-          y[0] = widen2<false>(Q(), k[a][t][0]);
-          y[1] = widen2<true>(Q(), k[a][t][0]);
-          y[2] = widen2<false>(Q(), k[a][t][1]);
-          y[3] = widen2<true>(Q(), k[a][t][1]);
-        } else {
-          y = k[a][t];
+      for (uint32_t t = 0; t < kLoads; ++t) {
+        uint32_t d;
+        const uint32_t keep = chunk(t, g, dim, d) ? ~0u : 0u;
+#pragma unroll
+        for (int h = 0; h < kDeep; ++h) {
+          u32x4 y;
+          if constexpr (kElem == 1) {
+            y[0] = widen2<false>(Q(), k[a][t][2 * h]);
+            y[1] = widen2<true>(Q(), k[a][t][2 * h]);
+            y[2] = widen2<false>(Q(), k[a][t][2 * h + 1]);
+            y[3] = widen2<true>(Q(), k[a][t][2 * h + 1]);
+          } else {
+            y = k[a][t];
+          }
+          if (!FULL) y &= keep;
+          x = mfma(Q(), y, q[t][h], x);
         }
-        if (!FULL) {
-          uint32_t d;
-          const uint32_t keep = chunk(t, g, dim, d) ? ~0u : 0u;
-          y &= keep;
-        }
-        x = mfma(Q(), y, q[t], x);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[4 * a + i] = x[i];
@@ -189,14 +200,11 @@ struct Engine16 {
 
   // Word w (values 2 w and 2 w + 1) of token i's values in panel p.
   __device__ __forceinline__ uint32_t word(int i, int p, int w) const {
-    if constexpr (kElem == 1) {
-      uint32_t x;
-      if constexpr (kVec == 4) x = v[i][p];
-      else x = v[i][p][w >> 1];
-      return w & 1 ? widen2<true>(Q(), x) : widen2<false>(Q(), x);
-    } else {
-      return v[i][p][w];
-    }
+    uint32_t x;
+    if constexpr (kVec * kElem <= 4) x = v[i][p];
+    else x = v[i][p][kElem == 1 ? w >> 1 : w];
+    if constexpr (kElem == 1) return w & 1 ? widen2<true>(Q(), x) : widen2<false>(Q(), x);
+    else return x;
   }
 
   // O += P V. A numerator is held as the sum of two 16-bit values, the
@@ -238,13 +246,15 @@ struct Engine32 {
   using Q = F32;
   using KV = F32;
   static constexpr int kElem = 4;
+  static constexpr int kDim = DIM;
   static constexpr int kGroup = 4, kTile = 16, kProducts = 1;
   static constexpr int kSteps = DIM / 16;
-  static constexpr int kVec = 4, kPanels = DIM / 64;
+  static constexpr int kVec = DIM % 64 ? 2 : 4, kPanels = DIM / (16 * kVec);
+  using VRaw = float __attribute__((ext_vector_type(kVec)));
 
   f32x4 q[kSteps];
   f32x4 k[kProducts][kSteps];
-  f32x4 v[kGroup][kPanels];
+  VRaw v[kGroup][kPanels];
   f32x4 o[kPanels][kVec];
 
   __device__ __forceinline__ static bool chunk(uint32_t s, uint32_t g, uint32_t dim, uint32_t& d) {
@@ -254,20 +264,13 @@ struct Engine32 {
     return false;
   }
 
-  __device__ __forceinline__ void load_q(const float* row, uint32_t g, uint32_t dim, bool live, bool wide) {
+  __device__ __forceinline__ void load_q(const float* row, uint32_t g, uint32_t dim, bool live) {
 #pragma unroll
     for (uint32_t s = 0; s < kSteps; ++s) {
       uint32_t d;
       const bool has = chunk(s, g, dim, d) && live;
       f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (has) {
-        if (wide) {
-          x = *reinterpret_cast<const f32x4*>(row + d);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = row[d + i];
-        }
-      }
+      if (has) __builtin_memcpy(&x, row + d, 16);
       q[s] = x;
     }
   }
@@ -277,7 +280,7 @@ struct Engine32 {
     for (uint32_t s = 0; s < kSteps; ++s) {
       uint32_t d;
       chunk(s, g, dim, d);
-      k[a][s] = load_raw<f32x4>(row + d * kElem);
+      k[a][s] = load_key<f32x4>(row + d * kElem);
     }
   }
 
@@ -285,12 +288,14 @@ struct Engine32 {
 #pragma unroll
     for (uint32_t p = 0; p < kPanels; ++p) {
       const uint32_t d = (p * 16u + c) * kVec;
-      v[i][p] = load_raw<f32x4>(row + (FULL || d < dim ? d : 0u) * kElem);
+      v[i][p] = load_value<VRaw>(row + (FULL || d < dim ? d : 0u) * kElem);
     }
   }
-  __device__ __forceinline__ void drop_v(int i) {
+  __device__ __forceinline__ void keep_v(int i, bool keep) {
 #pragma unroll
-    for (int p = 0; p < kPanels; ++p) v[i][p] = f32x4(0.0f);
+    for (int p = 0; p < kPanels; ++p)
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) v[i][p][j] = keep ? v[i][p][j] : 0.0f;
   }
 
   __device__ __forceinline__ void scores(float* s, uint32_t g, uint32_t dim) const {
