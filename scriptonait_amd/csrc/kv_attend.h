@@ -490,81 +490,90 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
   }
 }
 
-// The answers of requests that several ranges share. A workgroup takes 64
-// values of a query head, 16 partial answers at a time; the joining order
-// depends on their number alone.
+// The answers of requests that several ranges share. Row y of the grid is the
+// boundary before range y + 1. All boundaries inside a request take equal
+// parts of its value quads (of all query heads), so that a request of more
+// parts has more workgroups; in a workgroup neighbouring threads take
+// neighbouring quads, and where that leaves threads over, they take other
+// parts of the same quads. The order of joining follows from the number of
+// parts alone.
 template <class Q, class KV>
 __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
-  constexpr uint32_t kShare = 16;
-  __shared__ float s_m[kShare], s_l[kShare];
+  constexpr uint32_t kBatch = 8;
+  __shared__ float s_m[256], s_l[256];
   __shared__ f32x4 s_o[256];
-  const uint32_t tid = threadIdx.x, share = tid >> 4, chunks = (a.dim + 63u) / 64u;
-  const uint32_t qh = blockIdx.x / chunks, chunk = blockIdx.x % chunks, d = chunk * 64u + (tid & 15u) * 4u;
+  const Cut cut = reinterpret_cast<const Cut*>(a.workspace)[blockIdx.y + 1u];
+  if (cut.request == kNoId) return;
+  const uint32_t tid = threadIdx.x, n = cut.last - cut.first + 1u, quads = a.q_heads * (a.dim / 4u);
+  const uint32_t groups = (n - 1u) * gridDim.x, mine = (blockIdx.y - cut.first) * gridDim.x + blockIdx.x;
+  uint32_t width = 8u;  // quads of a workgroup: a power of 2
+  while (width < 256u && width * groups < quads) width *= 2u;
+  const uint32_t quad = mine * width + (tid & (width - 1u)), shares = 256u / width, share = tid / width;
+  if (mine * width >= quads) return;
+  const uint32_t x = min(quad, quads - 1u) * 4u, qh = a.by_dim.div(x), d = x - qh * a.dim;
   const uint32_t head = qh / a.group, in_group = qh % a.group, vhead = head * a.blocks + in_group / 16u;
   const uint32_t group = min(16u, a.group - in_group / 16u * 16u), qi = in_group % 16u;
-  const float vscale = KV::kId == LLMHIP_E4M3 ? a.scale[1][head] : 1.0f;
-  for (uint32_t r = 1u + blockIdx.y; r < a.ranges; r += gridDim.y) {
-    const Cut cut = reinterpret_cast<const Cut*>(a.workspace)[r];
-    if (cut.request == kNoId || cut.first + 1u != r) continue;  // the request's first range boundary joins it
-    const uint32_t n = cut.last - cut.first + 1u;
-    float m = -INFINITY, l = 0.0f;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (uint32_t k0 = share; k0 < n; k0 += 4u * kShare) {
-      float pm[4], pl[4];
-      f32x4 po[4];
+  const uint32_t at_o = qi * a.dim + d, at_m = group * a.dim + qi, at_l = at_m + group;
+  float m = -INFINITY, l = 0.0f;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (uint32_t k0 = share; k0 < n; k0 += kBatch * shares) {
+    float pm[kBatch], pl[kBatch];
+    f32x4 po[kBatch];
 #pragma unroll
-      for (uint32_t j = 0; j < 4u; ++j) {
-        const uint32_t k = k0 + j * kShare;
-        pm[j] = -INFINITY;
-        pl[j] = 0.0f;
-        po[j] = o * 0.0f;
-        if (k < n) {
-          const float* part =
-              a.workspace + a.part_offset + (((uint64_t)(cut.first + k) * a.vheads + vhead) * 2u + (k ? 0u : 1u)) * a.part_words;
-          pm[j] = part[group * a.dim + qi];
-          pl[j] = part[group * (a.dim + 1u) + qi];
-          if (d < a.dim) po[j] = *reinterpret_cast<const f32x4*>(part + qi * a.dim + d);
-        }
-      }
-      const float next = fmaxf(m, fmaxf(fmaxf(pm[0], pm[1]), fmaxf(pm[2], pm[3]))), top = next == -INFINITY ? 0.0f : next;
-      const float keep = __builtin_amdgcn_exp2f(m - top);
-      o *= keep;
-      l *= keep;
+    for (uint32_t j = 0; j < kBatch; ++j) {  // (the first one again where there is no more)
+      const uint32_t k = k0 + j * shares < n ? k0 + j * shares : k0;
+      const float* part =
+          a.workspace + a.part_offset + (((uint64_t)(cut.first + k) * a.vheads + vhead) * 2u + (k ? 0u : 1u)) * a.part_words;
+      pm[j] = part[at_m];
+      pl[j] = part[at_l];
+      po[j] = *reinterpret_cast<const f32x4*>(part + at_o);
+    }
+    float next = m;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float w = __builtin_amdgcn_exp2f(pm[j] - top);
-        l += pl[j] * w;
-        o += po[j] * w;
-      }
-      m = next;
+    for (uint32_t j = 0; j < kBatch; ++j) {
+      pm[j] = k0 + j * shares < n ? pm[j] : -INFINITY;
+      next = fmaxf(next, pm[j]);
     }
-    __syncthreads();
-    if ((tid & 15u) == 0u) {
-      s_m[share] = m;
-      s_l[share] = l;
+    const float top = next == -INFINITY ? 0.0f : next, keep = __builtin_amdgcn_exp2f(m - top);
+    o *= keep;
+    l *= keep;
+#pragma unroll
+    for (uint32_t j = 0; j < kBatch; ++j) {
+      const float w = __builtin_amdgcn_exp2f(pm[j] - top);
+      l += pl[j] * w;
+      o += po[j] * w;
     }
+    m = next;
+  }
+  if (shares > 1u) {
+    s_m[tid] = m;
+    s_l[tid] = l;
     s_o[tid] = o;
     __syncthreads();
-    if (share == 0u) {
-      for (uint32_t k = 0; k < kShare; ++k) m = fmaxf(m, s_m[k]);
-      const float top = m == -INFINITY ? 0.0f : m;
-      l = 0.0f;
-      o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-      for (uint32_t k = 0; k < kShare; ++k) {
-        const float w = __builtin_amdgcn_exp2f(s_m[k] - top);
-        l += s_l[k] * w;
-        o += s_o[k * 16u + tid] * w;
-      }
-      const float inv = l == 0.0f ? 0.0f : vscale / l;
-      typename Q::Raw* out =
-          static_cast<typename Q::Raw*>(a.out) + (int64_t)cut.request * a.out_stride[0] + (int64_t)qh * a.out_stride[1];
-      if (d < a.dim) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) out[d + j] = Q::store(o[j] * inv);
-      }
-      if (a.lse && tid == 0u && chunk == 0u) a.lse[(uint64_t)cut.request * a.q_heads + qh] = lse_of(m, l);
+    if (share) return;
+    float top = m;
+    for (uint32_t k = 1; k < shares; ++k) top = fmaxf(top, s_m[k * width + tid]);
+    const float whole = top;
+    top = top == -INFINITY ? 0.0f : top;
+    const float keep = __builtin_amdgcn_exp2f(m - top);
+    l *= keep;
+    o *= keep;
+    for (uint32_t k = 1; k < shares; ++k) {
+      const float w = __builtin_amdgcn_exp2f(s_m[k * width + tid] - top);
+      l += s_l[k * width + tid] * w;
+      o += s_o[k * width + tid] * w;
     }
+    m = whole;
   }
+  if (quad >= quads) return;
+  const float vscale = KV::kId == LLMHIP_E4M3 ? a.scale[1][head] : 1.0f, inv = l == 0.0f ? 0.0f : vscale / l;
+  Pack<Q, 4> y;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y.v[j] = Q::store(o[j] * inv);
+  typename Q::Raw* out =
+      static_cast<typename Q::Raw*>(a.out) + (int64_t)cut.request * a.out_stride[0] + (int64_t)qh * a.out_stride[1] + d;
+  __builtin_memcpy(out, y.v, sizeof y.v);
+  if (a.lse && d == 0u) a.lse[(uint64_t)cut.request * a.q_heads + qh] = lse_of(m, l);
 }
 
 template <class E, bool GROUPED>
@@ -583,8 +592,8 @@ hipError_t launch_attend_group(AttendArgs a, hipStream_t s) {
   hipLaunchKernelGGL((attend_kernel<E, GROUPED>), grid, threads, lds, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.ranges < 2u) return e;
-  hipLaunchKernelGGL((join_kernel<typename E::Q, typename E::KV>),
-                     dim3(a.q_heads * ((a.dim + 63u) / 64u), min(a.ranges - 1u, 64u)), dim3(256), 0, s, a);
+  const uint32_t quads = a.q_heads * (a.dim / 4u);
+  hipLaunchKernelGGL((join_kernel<typename E::Q, typename E::KV>), dim3((quads + 255u) / 256u, a.ranges - 1u), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
