@@ -119,8 +119,8 @@ int llmhip_kv_plan(llmhip_ctx* ctx, size_t pages, size_t page, int32_t* ring, co
  *
  *   dtype      of k, v, q and out_q: F32, BF16 or F16; the cache's is the
  *              same or E4M3
- *   k, v       device [T][heads][head_dim], strides (token, head) in
- *              elements; rows are dense. Slices of one packed projection
+ *   k, v       device [T][heads][head_dim], a token's and a head's stride
+ *              in elements; rows are dense. Slices of one packed projection
  *              output are such views
  *   slots      device [T]: llmhip_kv_plan's. A token of slot < 0 (padding)
  *              writes no key or value. Two tokens of one call must not share
@@ -136,9 +136,10 @@ int llmhip_kv_plan(llmhip_ctx* ctx, size_t pages, size_t page, int32_t* ring, co
  * A slot past the pool is skipped and flagged.
  */
 int llmhip_kv_append(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dtype, size_t T, const void* k,
-                     const int64_t k_stride[2], const void* v, const int64_t v_stride[2], const int64_t* slots,
-                     size_t q_heads, const void* q, const int64_t q_stride[2], void* out_q,
-                     const int64_t out_q_stride[2], const int32_t* positions, const llmhip_rope* rope, void* stream);
+                     int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                     const int64_t* slots, size_t q_heads, const void* q, int64_t q_token, int64_t q_head, void* out_q,
+                     int64_t out_q_token, int64_t out_q_head, const int32_t* positions, const llmhip_rope* rope,
+                     void* stream);
 
 /* Bytes of workspace that llmhip_kv_attend takes for this cache and q_heads,
  * whatever the batch. */
@@ -153,7 +154,8 @@ int llmhip_kv_attend_workspace(llmhip_ctx* ctx, const llmhip_kv_cache* cache, si
  * zeros and an lse of -inf.
  *
  *   dtype      of q and out: the cache's, or BF16 or F16 with an E4M3 cache
- *   q, out     device [B][q_heads][head_dim], strides (request, head)
+ *   q, out     device [B][q_heads][head_dim], a request's and a head's stride
+ *              in elements
  *   table      device [B][table_ld] page ids, table_pages of them used
  *   lens       device [B], with the newest token
  *   out_lse    device nullable [B][q_heads] f32
@@ -166,10 +168,9 @@ int llmhip_kv_attend_workspace(llmhip_ctx* ctx, const llmhip_kv_cache* cache, si
  * Scores, maxima, sums and outputs are accumulated in binary32.
  */
 int llmhip_kv_attend(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dtype, size_t B, size_t q_heads,
-                     const void* q, const int64_t q_stride[2], const int32_t* table, size_t table_pages,
-                     size_t table_ld, const int32_t* lens, size_t window, float scale, void* out,
-                     const int64_t out_stride[2], float* out_lse, void* workspace, size_t workspace_bytes,
-                     void* stream);
+                     const void* q, int64_t q_request, int64_t q_head, const int32_t* table, size_t table_pages,
+                     size_t table_ld, const int32_t* lens, size_t window, float scale, void* out, int64_t out_request,
+                     int64_t out_head, float* out_lse, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -38,6 +38,12 @@ int launched(hipError_t e, const char* what) {
 #define SUPPORTED(cond, what) \
   if (!(cond)) return unsupported(what)
 
+// Two arrays of n values are one and the same, or apart.
+bool same_or_apart(const int32_t* x, const int32_t* y, size_t n) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+  return a == b || a + n * sizeof(int32_t) <= b || b + n * sizeof(int32_t) <= a;
+}
+
 constexpr size_t kMaxInt = 0x7fffffff;
 constexpr size_t kMaxBatch = 65535;
 constexpr size_t kMaxHeads = 65535;
@@ -135,6 +141,8 @@ int llmhip_kv_plan(llmhip_ctx* ctx, size_t pages, size_t page, int32_t* ring, co
   ARG(T == 0 || (slots && positions), "slots and positions are required");
   SUPPORTED(R <= kMaxInt - 1024 && T <= kMaxInt - 1024, "R or T too large");
   TRY(check_table(table_pages, table_ld, page));
+  ARG(same_or_apart(lens, out_lens, R), "lens and out_lens overlap");
+  ARG(same_or_apart(free_state, out_free_state, 2), "free_state and out_free_state overlap");
   ON_DEVICE(info);
   PlanArgs a{};
   a.ring = ring;
@@ -161,9 +169,10 @@ int llmhip_kv_plan(llmhip_ctx* ctx, size_t pages, size_t page, int32_t* ring, co
 }
 
 int llmhip_kv_append(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dtype, size_t T, const void* k,
-                     const int64_t k_stride[2], const void* v, const int64_t v_stride[2], const int64_t* slots,
-                     size_t q_heads, const void* q, const int64_t q_stride[2], void* out_q,
-                     const int64_t out_q_stride[2], const int32_t* positions, const llmhip_rope* rope, void* stream) {
+                     int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                     const int64_t* slots, size_t q_heads, const void* q, int64_t q_token, int64_t q_head, void* out_q,
+                     int64_t out_q_token, int64_t out_q_head, const int32_t* positions, const llmhip_rope* rope,
+                     void* stream) {
   TRY(check_cache(cache));
   TRY(check_dtype(cache, dtype));
   ARG((q == nullptr) == (out_q == nullptr) && (q == nullptr) == (q_heads == 0), "q, out_q and q_heads go together");
@@ -173,13 +182,14 @@ int llmhip_kv_append(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
   const uint32_t dims = rope ? rope->dims : 0u;
   SUPPORTED(T <= kMaxInt - 1024 && q_heads <= kMaxHeads, "T or q_heads too large");
   if (T == 0) return LLMHIP_OK;
-  ARG(k && v && slots && k_stride && v_stride, "k, v, slots and their strides are required");
-  ARG(!q || (q_stride && out_q_stride), "q_stride and out_q_stride are required");
+  ARG(k && v && slots, "k, v and slots are required");
   ARG(!dims || positions, "positions are required with rope");
   // The widest access that the rows' starts and the pairs' places allow: 8
   // values (16 bytes of 16-bit types), 4, or single ones.
   const uint32_t elem = size_of(dtype), kv_elem = size_of(cache->dtype), dim = cache->head_dim;
   const bool neighbours = rope && rope->style == LLMHIP_ROPE_NEIGHBOURS;
+  const int64_t k_stride[2] = {k_token, k_head}, v_stride[2] = {v_token, v_head}, q_stride[2] = {q_token, q_head},
+                out_q_stride[2] = {out_q_token, out_q_head};
   uint32_t vec = 8;
   for (; vec > 1; vec = vec == 8 ? 4 : 1) {
     const uint32_t bytes = vec * elem, kv_bytes = vec * kv_elem;
@@ -227,10 +237,9 @@ int llmhip_kv_attend_workspace(llmhip_ctx* ctx, const llmhip_kv_cache* cache, si
 }
 
 int llmhip_kv_attend(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dtype, size_t B, size_t q_heads,
-                     const void* q, const int64_t q_stride[2], const int32_t* table, size_t table_pages,
-                     size_t table_ld, const int32_t* lens, size_t window, float scale, void* out,
-                     const int64_t out_stride[2], float* out_lse, void* workspace, size_t workspace_bytes,
-                     void* stream) {
+                     const void* q, int64_t q_request, int64_t q_head, const int32_t* table, size_t table_pages,
+                     size_t table_ld, const int32_t* lens, size_t window, float scale, void* out, int64_t out_request,
+                     int64_t out_head, float* out_lse, void* workspace, size_t workspace_bytes, void* stream) {
   TRY(check_cache(cache));
   TRY(check_dtype(cache, dtype));
   ARG(cache->dtype != LLMHIP_E4M3 || dtype != LLMHIP_F32, "dtype beside an E4M3 cache is BF16 or F16");
@@ -238,7 +247,7 @@ int llmhip_kv_attend(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
   SUPPORTED(q_heads <= kMaxHeads && B <= kMaxBatch, "B or q_heads too large");
   TRY(check_table(table_pages, table_ld, cache->page));
   if (B == 0) return LLMHIP_OK;
-  ARG(q && out && lens && q_stride && out_stride, "q, out, lens and their strides are required");
+  ARG(q && out && lens, "q, out and lens are required");
   ARG(table || table_pages == 0, "table is null");
   ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be given, aligned to 16 bytes");
   ON_DEVICE(info);
@@ -251,8 +260,10 @@ int llmhip_kv_attend(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
   set_pools(cache, a.pool, a.scale, a.pool_stride);
   a.table = table;
   a.lens = lens;
-  memcpy(a.q_stride, q_stride, sizeof a.q_stride);
-  memcpy(a.out_stride, out_stride, sizeof a.out_stride);
+  a.q_stride[0] = q_request;
+  a.q_stride[1] = q_head;
+  a.out_stride[0] = out_request;
+  a.out_stride[1] = out_head;
   a.table_ld = table_ld;
   a.workspace = static_cast<float*>(workspace);
   a.B = (uint32_t)B;

@@ -3,9 +3,14 @@
 //
 // Requests are served in order, so what request r gets follows from sums
 // over the requests before it: of their tokens, of the pages that they need
-// and of the pages that they give back. One workgroup forms the three prefix
-// sums, 1024 requests at a time, in 64 bits; each token of the chunk then
-// finds its request by bisection of the sums in LDS.
+// and of the pages that they give back. Every workgroup forms the three
+// prefix sums, 1024 requests at a time, in 64 bits, rather than waiting for one
+// that does; each then takes a part of the tokens, which find their request
+// by bisection of the sums in LDS, and of the released requests. Nothing that
+// one workgroup writes is read by another: a new page's id comes from the
+// ring, not from the table, and ids go back to the ring behind the free ones.
+// What bounds it is latency: two rounds of dependent reads and three
+// barriers for each 1024 requests.
 #include "kv_args.h"
 #include "wave_ops.h"
 
@@ -64,7 +69,8 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     count = 0u;
   }
   uint64_t asked = 0, needed = 0, returned = 0, taken = 0;
-  if (tid == 0u) a.start[0] = 0;
+  const bool sums = a.requests && blockIdx.x == 0u;  // this workgroup writes what is one value a request
+  if (sums && tid == 0u) a.start[0] = 0;
   for (uint32_t r0 = 0; r0 < a.R; r0 += kThreads) {
     const uint32_t r = r0 + tid, m = min(kThreads, a.R - r0);
     uint32_t base = 0, back = 0;
@@ -98,22 +104,28 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     s_back[tid] = back;
     s_put[tid] = (uint32_t)((head + count + put) % a.pages);
     s_ok[tid] = ok;
-    if (r < a.R) {
+    if (sums && r < a.R) {
       a.out_lens[r] = (int32_t)(base + (ok ? (uint32_t)n : 0u));
       a.granted[r] = ok ? (int32_t)n : 0;
       a.start[r + 1u] = (int32_t)(uint32_t)end;
     }
     __syncthreads();
 
-    // Released pages, read before a new page may take their place in the table.
-    for (uint32_t i = tid >> 6; i < m; i += kWaves) {
-      int32_t* row = a.table + (uint64_t)(r0 + i) * a.table_ld;
-      for (uint32_t p = tid & 63u; p < s_back[i]; p += 64u) a.ring[((uint64_t)s_put[i] + p) % a.pages] = row[p];
+    // Released pages. A request that is released and prompted anew gets its
+    // new pages here as well, each place read before it is written.
+    if (a.release && a.requests) {
+      for (uint32_t i = blockIdx.x * kWaves + (tid >> 6); i < m; i += gridDim.x * kWaves) {
+        const uint32_t back_i = s_back[i], fresh = back_i ? s_took[i] : 0u;
+        int32_t* row = a.table + (uint64_t)(r0 + i) * a.table_ld;
+        for (uint32_t p = tid & 63u; p < max(back_i, fresh); p += 64u) {
+          if (p < back_i) a.ring[((uint64_t)s_put[i] + p) % a.pages] = row[p];
+          if (p < fresh) row[p] = a.ring[((uint64_t)s_first[i] + p) % a.pages];
+        }
+      }
     }
-    __syncthreads();
 
     const uint32_t lo = (uint32_t)min(asked, (uint64_t)a.T), hi = (uint32_t)min(asked + n_sum, (uint64_t)a.T);
-    for (uint32_t t = lo + tid; t < hi; t += kThreads) {
+    for (uint32_t t = lo + blockIdx.x * kThreads + tid; a.tokens && t < hi; t += gridDim.x * kThreads) {
       uint32_t i = 0, above = m;  // the first request whose sum passes t
       while (i < above) {
         const uint32_t mid = (i + above) >> 1;
@@ -129,7 +141,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
         int32_t id;
         if (p >= have_i) {
           id = a.ring[((uint64_t)s_first[i] + (p - have_i)) % a.pages];
-          if (pos == p * a.page) *entry = id;  // a page's first token enters it
+          if (pos == p * a.page && !s_back[i]) *entry = id;  // a page's first token enters it
         } else {
           id = *entry;
         }
@@ -157,11 +169,12 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     __syncthreads();
   }
 
-  for (uint32_t t = (uint32_t)min(asked, (uint64_t)a.T) + tid; t < a.T; t += kThreads) {
+  for (uint32_t t = (uint32_t)min(asked, (uint64_t)a.T) + blockIdx.x * kThreads + tid; a.tokens && t < a.T;
+       t += gridDim.x * kThreads) {
     a.slots[t] = -1;
     a.positions[t] = 0;
   }
-  if (tid == 0u) {
+  if (sums && tid == 0u) {
     const uint64_t left = count - taken + returned;
     bad = bad || left > a.pages;  // pages came back that were free already
     a.out_free_state[0] = (int32_t)((head + taken) % a.pages);
@@ -172,8 +185,22 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
 
 }  // namespace
 
-hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), 0, s, a);
+hipError_t launch_kv_plan(PlanArgs a, hipStream_t s) {
+  // A thread for each token, a wave for each 8 requests (few are released).
+  const uint32_t groups = min(max(max((a.T + kThreads - 1u) / kThreads, (a.R + 127u) / 128u), 1u), 256u);
+  a.tokens = a.requests = true;
+  if (groups > 1u && (a.lens == a.out_lens || a.free_state == a.out_free_state)) {
+    // What every workgroup reads is to change in place: the tokens first.
+    a.requests = false;
+    hipLaunchKernelGGL(plan_kernel, dim3(groups), dim3(kThreads), 0, s, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    a.tokens = false;
+    a.requests = true;
+    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), 0, s, a);
+  } else {
+    hipLaunchKernelGGL(plan_kernel, dim3(groups), dim3(kThreads), 0, s, a);
+  }
   return hipGetLastError();
 }
 

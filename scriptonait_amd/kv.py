@@ -33,9 +33,9 @@ F32, BF16, F16, E4M3 = 0, 1, 2, 3
 DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.float8_e4m3fn: E4M3}
 EXPORTED_SYMBOLS = ("llmhip_kv_plan", "llmhip_kv_append", "llmhip_kv_attend_workspace", "llmhip_kv_attend")
 STYLES = {"halves": 0, "neighbours": 1}
+_NO_ROWS = (None, 0, 0)
 
 _vp, _sz, _u32, _i64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint32, ctypes.c_int64
-_Stride = _i64 * 2
 
 
 class LlmhipKvCache(ctypes.Structure):
@@ -60,13 +60,13 @@ def load_kv() -> ctypes.CDLL:
         lib.llmhip_kv_plan.argtypes = [_vp, _sz, _sz, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _sz,
                                        _vp, _vp, _vp, _vp]
         lib.llmhip_kv_append.restype = ctypes.c_int
-        lib.llmhip_kv_append.argtypes = [_vp, _vp, _u32, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp, _vp, _vp, _vp,
-                                         _vp, _vp]
+        rows = [_vp, _i64, _i64]
+        lib.llmhip_kv_append.argtypes = [_vp, _vp, _u32, _sz, *rows, *rows, _vp, _sz, *rows, *rows, _vp, _vp, _vp]
         lib.llmhip_kv_attend_workspace.restype = ctypes.c_int
         lib.llmhip_kv_attend_workspace.argtypes = [_vp, _vp, _sz, ctypes.POINTER(_sz)]
         lib.llmhip_kv_attend.restype = ctypes.c_int
-        lib.llmhip_kv_attend.argtypes = [_vp, _vp, _u32, _sz, _sz, _vp, _vp, _vp, _sz, _sz, _vp, _sz, ctypes.c_float,
-                                         _vp, _vp, _vp, _vp, _sz, _vp]
+        lib.llmhip_kv_attend.argtypes = [_vp, _vp, _u32, _sz, _sz, *rows, _vp, _sz, _sz, _vp, _sz, ctypes.c_float, *rows,
+                                         _vp, _vp, _sz, _vp]
         _lib = lib
     return _lib
 
@@ -76,31 +76,57 @@ def _check(lib, status: int) -> None:
         raise SamplerError(status, lib.llmhip_last_error().decode(errors="replace"))
 
 
-def _vector(t, n: Optional[int], dtype, name: str, device):
+# A small call's time is the host's, so the checks below ask a tensor for each
+# thing once and format nothing before they fail.
+def _vector(t, n: int, dtype, name: str, device) -> int:
     """A dense device vector of n values; its address."""
-    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{name} must be a contiguous {dtype} vector" + ("" if n is None else f" of {n} values"))
+    if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} vector of {n} values")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
     return t.data_ptr()
 
 
-def _table(t, n: int, device) -> int:
-    """A block table of n requests; its row stride."""
-    if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != n or (t.stride(1) != 1 and t.shape[1] > 1 and n):
+def _rows(t, shape, dtype, name: str, device):
+    """A tensor of `shape` whose last dimension is dense; its address and its
+    other strides."""
+    a, b, c = t.stride() if t.dim() == 3 else (0, 0, 0)
+    if t.shape != shape or t.dtype is not dtype or (c != 1 and shape[0]):
+        raise ValueError(f"{name} must be {dtype} {list(shape)} with dense rows")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
+    return t.data_ptr(), a, b
+
+
+def _table(t, n: int, device):
+    """A block table of n requests; its address, pages and row stride."""
+    if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != n or (t.stride(1) != 1 and t.shape[1] > 1 and n):
         raise ValueError(f"table must be an int32 [{n}, pages] tensor with dense rows")
     if t.device != device:
         raise ValueError(f"table is on {t.device}, not on {device}")
-    return t.stride(0) if n > 1 else t.shape[1]
+    pages = t.shape[1]
+    return t.data_ptr(), pages, t.stride(0) if n > 1 else pages
 
 
-def _stream(stream, device, *tensors) -> int:
-    if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
-    for t in tensors:  # their memory is not to be handed out again before this stream has used it
+def _on(stream, tensors) -> int:
+    """A stream of the caller's choice; the tensors' memory is not handed out
+    again before it has used them."""
+    for t in tensors:
         if t is not None:
             t.record_stream(stream)
     return stream.cuda_stream
+
+
+def _current(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+# torch.cuda.current_stream builds a Stream object for each call (about a
+# microsecond); this is the query beneath it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+if _raw_stream is not None:
+    def _current(device) -> int:  # noqa: F811
+        return _raw_stream(device.index)
 
 
 class Rope:
@@ -148,6 +174,7 @@ class PagePool:
         self._ring = _vector(free_ring, pages, torch.int32, "free_ring", self.device)
         self._state = _vector(free_state, 2, torch.int32, "free_state", self.device)
         self.free_ring, self.free_state = free_ring, free_state
+        self._plan = self.lib.llmhip_kv_plan
 
     def plan(self, lens, table, out_lens, granted, start, slots, positions, new_tokens=None, release=None,
              out_free_state=None, stream=None) -> None:
@@ -159,20 +186,19 @@ class PagePool:
         goes there."""
         dev, i32 = self.device, torch.int32
         R, T = lens.shape[0], slots.shape[0]
-        ld = _table(table, R, dev)
         state = self.free_state if out_free_state is None else out_free_state
-        status = self.lib.llmhip_kv_plan(
-            self.sampler.ctx, self.pages, self.page_size, self._ring, self._state, R,
-            _vector(lens, R, i32, "lens", dev),
+        status = self._plan(
+            self.sampler.ctx, self.pages, self.page_size, self._ring, self._state, R, _vector(lens, R, i32, "lens", dev),
             None if new_tokens is None else _vector(new_tokens, R, i32, "new_tokens", dev),
-            None if release is None else _vector(release, R, i32, "release", dev), table.data_ptr(), table.shape[1],
-            ld, _vector(out_lens, R, i32, "out_lens", dev),
-            _vector(granted, R, i32, "granted", dev), _vector(start, R + 1, i32, "start", dev), T,
-            _vector(slots, T, torch.int64, "slots", dev), _vector(positions, T, i32, "positions", dev),
-            _vector(state, 2, i32, "out_free_state", dev),
-            _stream(stream, dev, lens, new_tokens, release, table, out_lens, granted, start, slots, positions, state,
-                    self.free_ring, self.free_state))
-        _check(self.lib, status)
+            None if release is None else _vector(release, R, i32, "release", dev), *_table(table, R, dev),
+            _vector(out_lens, R, i32, "out_lens", dev), _vector(granted, R, i32, "granted", dev),
+            _vector(start, R + 1, i32, "start", dev), T, _vector(slots, T, torch.int64, "slots", dev),
+            _vector(positions, T, i32, "positions", dev),
+            self._state if out_free_state is None else _vector(out_free_state, 2, i32, "out_free_state", dev),
+            _current(dev) if stream is None else _on(stream, (lens, new_tokens, release, table, out_lens, granted, start,
+                                                              slots, positions, state, self.free_ring, self.free_state)))
+        if status:
+            _check(self.lib, status)
 
 
 class KVCache:
@@ -207,17 +233,11 @@ class KVCache:
         self._c = LlmhipKvCache(k_pool.data_ptr(), v_pool.data_ptr(), *scales, (_i64 * 3)(*k_pool.stride()[:3]),
                                 (_i64 * 3)(*v_pool.stride()[:3]), DTYPES[self.dtype], pages, page, heads, dim)
         self._ref = ctypes.addressof(self._c)
-
-    def _rows(self, t, n: int, heads: Optional[int], dtype, name: str):
-        """A [n, heads, head_dim] tensor with dense rows; its strides."""
-        shape, stride = t.shape, t.stride()
-        if (len(shape) != 3 or shape[0] != n or (heads is not None and shape[1] != heads) or shape[2] != self.head_dim
-                or (stride[2] != 1 and n) or t.dtype != dtype):
-            raise ValueError(f"{name} must be {dtype} [{n}, {'heads' if heads is None else heads}, {self.head_dim}] "
-                             "with dense rows")
-        if t.device != self.device:
-            raise ValueError(f"{name} is on {t.device}, not on {self.device}")
-        return _Stride(stride[0], stride[1])
+        self._scale = 1.0 / math.sqrt(dim)
+        self._append, self._attend = self.lib.llmhip_kv_append, self.lib.llmhip_kv_attend
+        # What may come beside this cache, as the C entries name it.
+        self._codes = {t: c for t, c in DTYPES.items()
+                       if c != E4M3 and (t is self.dtype or self.dtype is torch.float8_e4m3fn)}
 
     def append(self, k, v, slots, q=None, out_q=None, positions=None, rope: Optional[Rope] = None, stream=None) -> None:
         """llmhip_kv_append: k and v [T, heads, head_dim] into the slots ([T]
@@ -225,25 +245,36 @@ class KVCache:
         int32); with q [T, q_heads, head_dim] its rotated rows go to out_q
         (which may be q). k, v and q may be views of one packed tensor; their
         type is the cache's, or any of the wider ones beside a float8 cache."""
-        dt = k.dtype
-        T = k.shape[0]
-        if dt not in DTYPES or dt == torch.float8_e4m3fn or (dt != self.dtype and self.dtype != torch.float8_e4m3fn):
+        dt, dev = k.dtype, self.device
+        code = self._codes.get(dt)
+        if code is None:
             raise ValueError(f"k is {dt}, which does not go into a {self.dtype} cache")
         if (q is None) != (out_q is None):
             raise ValueError("q and out_q go together")
-        if rope is not None and (positions is None or rope.dims > self.head_dim):
+        T = k.shape[0]
+        shape = (T, self.heads, self.head_dim)
+        if rope is None:
+            turn = None
+        elif positions is None or rope.dims > self.head_dim:
             raise ValueError("rope needs positions, and dims of at most head_dim")
-        q_heads = 0 if q is None else q.shape[1]
-        status = self.lib.llmhip_kv_append(
-            self.sampler.ctx, self._ref, DTYPES[dt], T, k.data_ptr(), self._rows(k, T, self.heads, dt, "k"),
-            v.data_ptr(), self._rows(v, T, self.heads, dt, "v"), _vector(slots, T, torch.int64, "slots", self.device),
-            q_heads, None if q is None else q.data_ptr(), None if q is None else self._rows(q, T, None, dt, "q"),
-            None if q is None else out_q.data_ptr(),
-            None if q is None else self._rows(out_q, T, q_heads, dt, "out_q"),
-            None if positions is None else _vector(positions, T, torch.int32, "positions", self.device),
-            None if rope is None else rope._ref, _stream(stream, self.device, k, v, slots, q, out_q, positions,
-                                                         self.k_pool, self.v_pool, self.k_scale, self.v_scale))
-        _check(self.lib, status)
+        else:
+            turn = rope._ref
+        if q is None:
+            heads, q_rows, out_rows = 0, _NO_ROWS, _NO_ROWS
+        else:
+            if q.dim() != 3:
+                raise ValueError("q must be [T, q_heads, head_dim]")
+            heads = q.shape[1]
+            q_shape = (T, heads, self.head_dim)
+            q_rows, out_rows = _rows(q, q_shape, dt, "q", dev), _rows(out_q, q_shape, dt, "out_q", dev)
+        status = self._append(
+            self.sampler.ctx, self._ref, code, T, *_rows(k, shape, dt, "k", dev), *_rows(v, shape, dt, "v", dev),
+            _vector(slots, T, torch.int64, "slots", dev), heads, *q_rows, *out_rows,
+            None if positions is None else _vector(positions, T, torch.int32, "positions", dev), turn,
+            _current(dev) if stream is None else _on(stream, (k, v, slots, q, out_q, positions, self.k_pool, self.v_pool,
+                                                              self.k_scale, self.v_scale)))
+        if status:
+            _check(self.lib, status)
 
     def workspace(self, q_heads: int):
         """A workspace for attend with q_heads query heads, whatever the
@@ -260,26 +291,31 @@ class KVCache:
         like q, out_lse [B, q_heads] float32; scale defaults to
         head_dim ** -0.5. q_heads is a multiple of the cache's heads, and q
         of the cache's type (bfloat16 or float16 beside a float8 cache)."""
-        dt = q.dtype
-        if dt not in DTYPES or dt == torch.float8_e4m3fn or (dt != self.dtype and (
-                self.dtype != torch.float8_e4m3fn or dt == torch.float32)):
+        dt, dev = q.dtype, self.device
+        code = self._codes.get(dt)
+        if code is None or (dt is torch.float32 and self.dtype is not dt):
             raise ValueError(f"q is {dt}, which does not go with a {self.dtype} cache")
-        B, heads, dev = q.shape[0], q.shape[1], self.device
+        if q.dim() != 3:
+            raise ValueError("q must be [B, q_heads, head_dim]")
+        B, heads = q.shape[0], q.shape[1]
         if not heads or heads % self.heads:
             raise ValueError(f"q must have a multiple of {self.heads} heads")
-        ld = _table(table, B, dev)
         if window < 0:
             raise ValueError("window must not be negative")
-        if out_lse is not None and (out_lse.dtype != torch.float32 or out_lse.shape != q.shape[:2]
-                                    or not out_lse.is_contiguous() or out_lse.device != dev):
+        if out_lse is None:
+            lse = None
+        elif out_lse.dtype is not torch.float32 or out_lse.shape != (B, heads) or not out_lse.is_contiguous() \
+                or out_lse.device != dev:
             raise ValueError(f"out_lse must be a contiguous float32 [{B}, {heads}] tensor on {dev}")
-        status = self.lib.llmhip_kv_attend(
-            self.sampler.ctx, self._ref, DTYPES[dt], B, heads, q.data_ptr(), self._rows(q, B, heads, dt, "q"),
-            table.data_ptr(), table.shape[1], ld,
-            _vector(lens, B, torch.int32, "lens", dev), window,
-            1.0 / math.sqrt(self.head_dim) if scale is None else scale, out.data_ptr(),
-            self._rows(out, B, heads, dt, "out"), None if out_lse is None else out_lse.data_ptr(),
-            _vector(workspace, None, torch.uint8, "workspace", dev), workspace.numel(),
-            _stream(stream, dev, q, table, lens, out, out_lse, workspace, self.k_pool, self.v_pool, self.k_scale,
-                    self.v_scale))
-        _check(self.lib, status)
+        else:
+            lse = out_lse.data_ptr()
+        shape = (B, heads, self.head_dim)
+        size = workspace.numel()
+        status = self._attend(
+            self.sampler.ctx, self._ref, code, B, heads, *_rows(q, shape, dt, "q", dev), *_table(table, B, dev),
+            _vector(lens, B, torch.int32, "lens", dev), window, self._scale if scale is None else scale,
+            *_rows(out, shape, dt, "out", dev), lse, _vector(workspace, size, torch.uint8, "workspace", dev), size,
+            _current(dev) if stream is None else _on(stream, (q, table, lens, out, out_lse, workspace, self.k_pool,
+                                                              self.v_pool, self.k_scale, self.v_scale)))
+        if status:
+            _check(self.lib, status)

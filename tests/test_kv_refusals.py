@@ -70,15 +70,15 @@ CACHES = [
 
 
 def _attend(cache, dtype=kv.BF16, B=2, heads=8, q=SOME, table=SOME, P=4, ld=4, ws=SOME, window=0, ctx=None):
-    st = (ctypes.c_int64 * 2)(512, 64)
-    return kv.load_kv().llmhip_kv_attend(ctx, ctypes.byref(cache) if cache else None, dtype, B, heads, q, st, table, P, ld, SOME,
-                                         window, 0.1, SOME, st, None, ws, 1 << 40, None)
+    st = (512, 64)
+    return kv.load_kv().llmhip_kv_attend(ctx, ctypes.byref(cache) if cache else None, dtype, B, heads, q, *st, table, P, ld, SOME,
+                                         window, 0.1, SOME, *st, None, ws, 1 << 40, None)
 
 
 def _append(cache, dtype=kv.BF16, T=2, k=SOME, slots=SOME, heads=8, q=SOME, out_q=SOME, positions=SOME, rope=None, ctx=None):
-    st = (ctypes.c_int64 * 2)(512, 64)
-    return kv.load_kv().llmhip_kv_append(ctx, ctypes.byref(cache) if cache else None, dtype, T, k, st, SOME, st, slots, heads, q,
-                                         st, out_q, st, positions, None if rope is None else ctypes.byref(rope), None)
+    st = (512, 64)
+    return kv.load_kv().llmhip_kv_append(ctx, ctypes.byref(cache) if cache else None, dtype, T, k, *st, SOME, *st, slots, heads,
+                                         q, *st, out_q, *st, positions, None if rope is None else ctypes.byref(rope), None)
 
 
 @pytest.mark.parametrize("change,code,text", CACHES)
