@@ -9,7 +9,8 @@ struct Device {
   bool ok = false;
   explicit Device(int dev) {
     if (hipGetDevice(&prev) != hipSuccess) prev = -1;
-    ok = hipSetDevice(dev) == hipSuccess;
+    ok = prev == dev || hipSetDevice(dev) == hipSuccess;
+    if (prev == dev) prev = -1;  // nothing to set back
   }
   ~Device() {
     if (prev >= 0) (void)hipSetDevice(prev);

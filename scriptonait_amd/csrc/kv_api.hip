@@ -184,15 +184,16 @@ int llmhip_kv_append(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
   if (T == 0) return LLMHIP_OK;
   ARG(k && v && slots, "k, v and slots are required");
   ARG(!dims || positions, "positions are required with rope");
-  // The widest access that the rows' starts and the pairs' places allow: 8
-  // values (16 bytes of 16-bit types), 4, or single ones.
+  // The widest vectors that the rows' starts and the pairs' places allow: a
+  // vector of 16 bytes, or of 8, or single values; of neighbouring pairs two
+  // vectors are one access.
   const uint32_t elem = size_of(dtype), kv_elem = size_of(cache->dtype), dim = cache->head_dim;
   const bool neighbours = rope && rope->style == LLMHIP_ROPE_NEIGHBOURS;
   const int64_t k_stride[2] = {k_token, k_head}, v_stride[2] = {v_token, v_head}, q_stride[2] = {q_token, q_head},
                 out_q_stride[2] = {out_q_token, out_q_head};
-  uint32_t vec = 8;
-  for (; vec > 1; vec = vec == 8 ? 4 : 1) {
-    const uint32_t bytes = vec * elem, kv_bytes = vec * kv_elem;
+  uint32_t vec = (neighbours ? 8 : 16) / elem;
+  for (const uint32_t least = 8 / elem; vec >= least; vec /= 2) {
+    const uint32_t access = neighbours ? 2 * vec : vec, bytes = access * elem, kv_bytes = access * kv_elem;
     if (dims % (2 * vec) || (dim - dims) % (2 * vec)) continue;
     if (!rows_on(k, k_stride, 2, elem, bytes) || !rows_on(v, v_stride, 2, elem, bytes)) continue;
     if (q && (!rows_on(q, q_stride, 2, elem, bytes) || !rows_on(out_q, out_q_stride, 2, elem, bytes))) continue;
@@ -200,6 +201,7 @@ int llmhip_kv_append(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
         rows_on(cache->v_pool, cache->v_stride, 3, kv_elem, kv_bytes))
       break;
   }
+  if (vec < 8 / elem) vec = 1;
   ON_DEVICE(info);
   AppendArgs a{};
   a.x[0] = q;

@@ -77,7 +77,7 @@ struct AttendArgs {
   uint32_t* status;
 };
 
-hipError_t launch_kv_plan(PlanArgs a, hipStream_t s);
+hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s);
 hipError_t launch_kv_append(const AppendArgs& a, uint32_t dtype, uint32_t kv_dtype, bool neighbours, uint32_t vec,
                             hipStream_t s);
 hipError_t launch_attend_f32(const AttendArgs& a, hipStream_t s);
