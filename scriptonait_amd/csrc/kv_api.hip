@@ -180,7 +180,7 @@ int llmhip_kv_append(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
   ARG(!rope || rope->style <= LLMHIP_ROPE_NEIGHBOURS, "unknown rope style");
   ARG(!rope || (rope->dims % 2 == 0 && rope->dims <= cache->head_dim), "rope->dims must be even and at most head_dim");
   const uint32_t dims = rope ? rope->dims : 0u;
-  SUPPORTED(T <= kMaxInt - 1024 && q_heads <= kMaxHeads, "T or q_heads too large");
+  SUPPORTED(T <= ((size_t)1 << 23) && q_heads <= kMaxHeads, "T (over 2^23) or q_heads too large");
   if (T == 0) return LLMHIP_OK;
   ARG(k && v && slots, "k, v and slots are required");
   ARG(!dims || positions, "positions are required with rope");

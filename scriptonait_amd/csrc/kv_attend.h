@@ -234,25 +234,28 @@ struct Run {
 
   // A tile's scores and values into ref, sum and o.
   __device__ __forceinline__ void add(float* s, uint32_t seen) {
+    const bool edge = __any(seen != kAll);
+    float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < E::kGroup; ++i) s[i] *= scale;
-    if (__any(seen != kAll)) {
+    for (int i = 0; i < E::kGroup; ++i) {
+      const float x = s[i] * scale;
+      top = fmaxf(top, !edge || (seen >> i & 1u) ? x : -INFINITY);
+    }
+    if (__any(top > limit)) raise(top);
+    // The scaled score is not rounded before the reference is taken from it:
+    // only the difference is, and that is small where it counts.
+#pragma unroll
+    for (int i = 0; i < E::kGroup; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -ref));
+    if (edge) {
 #pragma unroll
       for (int i = 0; i < E::kGroup; ++i) {
         const bool keep = seen >> i & 1u;
-        s[i] = keep ? s[i] : -INFINITY;
+        s[i] = keep ? s[i] : 0.0f;
         e.keep_v(i, keep);
       }
     }
-    float top = s[0];
 #pragma unroll
-    for (int i = 1; i < E::kGroup; ++i) top = fmaxf(top, s[i]);
-    if (__any(top > limit)) raise(top);
-#pragma unroll
-    for (int i = 0; i < E::kGroup; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(s[i] - ref);
-      sum += s[i];
-    }
+    for (int i = 0; i < E::kGroup; ++i) sum += s[i];
     e.accumulate(s);
   }
 
@@ -579,8 +582,10 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
 template <class E, bool GROUPED>
 hipError_t launch_attend_group(AttendArgs a, hipStream_t s) {
   constexpr uint32_t kWaves = kWavesOf<E, GROUPED>;
+  // All waves have work: 12 heads are three teams of 4 with two waves each, not
+  // two of 6 with one (head size 96: 130 us and 135; 3 heads of 64: 17 and 19).
   a.team = kWaves;
-  while (a.vheads % a.team) --a.team;
+  while (a.vheads % a.team) a.team /= 2u;
   a.splits = kWaves / a.team;
   const uint32_t teams = a.vheads / a.team;
   // A workgroup of 8 waves, or two of 4, on each compute unit; more requests

@@ -129,6 +129,18 @@ def test_many_ragged_requests(sampler, q, kv):
     _check(c, _attend(sampler, c, 50, want_lse=False), 50)
 
 
+@pytest.mark.parametrize("q,kv", [("f32", "f32"), ("bf16", "bf16"), ("f16", "e4m3")])
+@pytest.mark.parametrize("B,Hq,Hkv,D,longest", [(2100, 2, 1, 64, 90), (65, 4, 4, 128, 300), (3, 2100, 2100, 8, 40),
+                                                (2, 96, 24, 32, 700)])
+def test_batches_and_heads_beyond_one_cut(sampler, q, kv, B, Hq, Hkv, D, longest):
+    """More requests than are cut into ranges, than a wave has lanes; more
+    heads than workgroups fill the card with, and teams of 8."""
+    rs = np.random.default_rng(B)
+    c = _make(B, rs.integers(0, longest, B), Hq, Hkv, D, 16, q, kv)
+    _check(c, _attend(sampler, c))
+    assert sampler.status().flags == 0
+
+
 @pytest.mark.parametrize("q,kv", PAIRS)
 @pytest.mark.parametrize("wide", [False, True])
 def test_wide_tables_and_long_requests_beside_short_ones(sampler, q, kv, wide):
