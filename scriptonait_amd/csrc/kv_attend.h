@@ -118,7 +118,9 @@ struct Cut {
   uint32_t request, first, last, unused;
 };
 
-template <class E, bool GROUPED>
+// GROUPED: pages are whole groups of tokens. ONCE: values are not found in a
+// cache again.
+template <class E, bool GROUPED, bool ONCE>
 struct Run {
   static constexpr int kIds = GROUPED ? 1 : E::kGroup;       // page ids of the lane's V tokens
   static constexpr int kKIds = GROUPED ? 1 : E::kProducts;   // and of its K tokens
@@ -175,10 +177,10 @@ struct Run {
       const char* p = token_row(1, x.v[0], a.by_page.mod(t));
       const int64_t step = a.pool_stride[1][1] * E::kElem;
 #pragma unroll
-      for (int i = 0; i < E::kGroup; ++i) e.load_v(i, p + i * step, c, a.dim);
+      for (int i = 0; i < E::kGroup; ++i) e.template load_v<ONCE>(i, p + i * step, c, a.dim);
     } else {
 #pragma unroll
-      for (int i = 0; i < E::kGroup; ++i) e.load_v(i, token_row(1, x.v[i], a.by_page.mod(t + i)), c, a.dim);
+      for (int i = 0; i < E::kGroup; ++i) e.template load_v<ONCE>(i, token_row(1, x.v[i], a.by_page.mod(t + i)), c, a.dim);
     }
   }
   // Which of the lane's tokens are seen, as bits; kAll in every lane of most tiles.
@@ -291,7 +293,7 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 // Words of a partial answer: o of every query head, then m, then l.
 __host__ __device__ __forceinline__ uint32_t partial_words(uint32_t group, uint32_t dim) { return group * (dim + 2u); }
 
-template <class E, bool GROUPED>
+template <class E, bool GROUPED, bool ONCE>
 __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(AttendArgs a) {
   constexpr uint32_t kWaves = kWavesOf<E, GROUPED>;
   extern __shared__ uint32_t s_mem[];
@@ -325,7 +327,7 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
   }
   if (bad && vhead == 0u && (range == 0u || !a.ranges)) atomicOr(a.status, LLMHIP_KSTATUS_BAD_INDEX);
 
-  Run<E, GROUPED> run(a);
+  Run<E, GROUPED, ONCE> run(a);
   run.g = lane >> 4;
   run.c = lane & 15u;
 #pragma unroll
@@ -579,7 +581,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
   if (a.lse && d == 0u) a.lse[(uint64_t)cut.request * a.q_heads + qh] = lse_of(m, l);
 }
 
-template <class E, bool GROUPED>
+template <class E, bool GROUPED, bool ONCE>
 hipError_t launch_attend_group(AttendArgs a, hipStream_t s) {
   constexpr uint32_t kWaves = kWavesOf<E, GROUPED>;
   // All waves have work: 12 heads are three teams of 4 with two waves each, not
@@ -617,7 +619,7 @@ hipError_t launch_attend_group(AttendArgs a, hipStream_t s) {
   a.start_words = a.ranges && a.B > 64u ? 16u + (a.B + 1u + 3u) / 4u * 4u : 0u;
   const uint32_t lds = (a.start_words + (a.splits > 1u ? 2u * kWaves * a.part_words : 0u)) * 4u;
   const dim3 grid((a.ranges ? a.ranges : a.B) * teams), threads(a.team * a.splits * 64u);
-  hipLaunchKernelGGL((attend_kernel<E, GROUPED>), grid, threads, lds, s, a);
+  hipLaunchKernelGGL((attend_kernel<E, GROUPED, ONCE>), grid, threads, lds, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.ranges < 2u) return e;
   const uint32_t quads = a.q_heads * (a.dim / 4u);
@@ -625,9 +627,20 @@ hipError_t launch_attend_group(AttendArgs a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// Values are read past the caches unless the next call may find them there (the
+// card keeps 256 MB: pools of up to 64 MiB each), or the heads beside them on
+// their cache lines do. 537 MB 99 us and 107 with plain loads, 2.2 GB of E4M3 345
+// and 378; 67 MB of one head 26.2 and 24.8, 205 MB of rows of 32 bytes 87 and 72.
 template <class E>
 hipError_t launch_attend_engine(const AttendArgs& a, hipStream_t s) {
-  return a.page % E::kGroup == 0u ? launch_attend_group<E, true>(a, s) : launch_attend_group<E, false>(a, s);
+  const bool grouped = a.page % E::kGroup == 0u;
+  if constexpr (E::kDim == 32) {
+    return grouped ? launch_attend_group<E, true, false>(a, s) : launch_attend_group<E, false, false>(a, s);
+  } else {
+    if (!grouped) return launch_attend_group<E, false, true>(a, s);
+    const uint64_t pool = (uint64_t)a.pages * a.page * a.heads * a.dim * E::kElem;
+    return pool > (64u << 20) ? launch_attend_group<E, true, true>(a, s) : launch_attend_group<E, true, false>(a, s);
+  }
 }
 
 // ENGINE<DIM, FULL>: the smallest DIM that holds head_dim. (Its name is part of

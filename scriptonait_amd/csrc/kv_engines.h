@@ -53,10 +53,11 @@ template <class T>
 __device__ __forceinline__ T load_key(const char* p) {
   return *reinterpret_cast<const T*>(p);
 }
-// Values: whole lines, used once.
-template <class T>
+// Values: whole lines; ONCE: past the caches' reach before they are read again.
+template <class T, bool ONCE>
 __device__ __forceinline__ T load_value(const char* p) {
-  return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+  if constexpr (ONCE) return __builtin_nontemporal_load(reinterpret_cast<const T*>(p));
+  else return *reinterpret_cast<const T*>(p);
 }
 
 // The 16-bit types' products, 32 deep.
@@ -150,11 +151,12 @@ struct Engine16 {
     }
   }
 
+  template <bool ONCE>
   __device__ __forceinline__ void load_v(int i, const char* row, uint32_t c, uint32_t dim) {
 #pragma unroll
     for (uint32_t p = 0; p < kPanels; ++p) {
       const uint32_t d = (p * 16u + c) * kVec;
-      v[i][p] = load_value<VRaw>(row + (FULL || d < dim ? d : 0u) * kElem);
+      v[i][p] = load_value<VRaw, ONCE>(row + (FULL || d < dim ? d : 0u) * kElem);
     }
   }
   __device__ __forceinline__ void keep_v(int i, bool keep) {
@@ -284,11 +286,12 @@ struct Engine32 {
     }
   }
 
+  template <bool ONCE>
   __device__ __forceinline__ void load_v(int i, const char* row, uint32_t c, uint32_t dim) {
 #pragma unroll
     for (uint32_t p = 0; p < kPanels; ++p) {
       const uint32_t d = (p * 16u + c) * kVec;
-      v[i][p] = load_value<VRaw>(row + (FULL || d < dim ? d : 0u) * kElem);
+      v[i][p] = load_value<VRaw, ONCE>(row + (FULL || d < dim ? d : 0u) * kElem);
     }
   }
   __device__ __forceinline__ void keep_v(int i, bool keep) {

@@ -60,12 +60,19 @@ def _cuda(x, layout=None):
     return y
 
 
-def _attend(sampler, c, window=0, scale=None, want_lse=True, q=None, out=None, stream=None):
+def _attend(sampler, c, window=0, scale=None, want_lse=True, q=None, out=None, stream=None, pool_bytes=0):
     import torch
 
     from scriptonait_amd.kv import KVCache
 
-    cache = KVCache(sampler, _cuda(c["k_pool"]), _cuda(c["v_pool"]), _cuda(c["k_scale"]), _cuda(c["v_scale"]))
+    pools = [_cuda(c["k_pool"]), _cuda(c["v_pool"])]
+    if pool_bytes:  # more pages behind those that are used
+        for i, p in enumerate(pools):
+            page = p[0].numel() * p.element_size()
+            raw = torch.full((pool_bytes // page + 1, page), 255, dtype=torch.uint8, device="cuda")
+            raw[:len(p)] = p.contiguous().view(torch.uint8).reshape(len(p), page)
+            pools[i] = raw.view(p.dtype).view(-1, *p.shape[1:])
+    cache = KVCache(sampler, *pools, _cuda(c["k_scale"]), _cuda(c["v_scale"]))
     q = _cuda(c["q"]) if q is None else q
     B, Hq, D = q.shape
     out = torch.full((B, Hq, D), 77.0, dtype=q.dtype, device="cuda") if out is None else out
@@ -237,6 +244,17 @@ def test_caches_past_32_bits(sampler):
     assert torch.equal(pools[0][N - 1, [page - 1, 0]], x) and torch.equal(pools[1][N - 1, [page - 1, 0]], -x)
     del pools, cache
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("q,kv", PAIRS)
+@pytest.mark.parametrize("D,page", [(64, 16), (80, 16), (128, 8), (256, 32), (192, 64), (128, 20)])
+def test_large_pools(sampler, q, kv, D, page):
+    """Pools that no cache of the card holds: their values are read another way."""
+    c = _make(D + page, [300, 0, 77, 33], 8, 4, D, page, q, kv)
+    got = _attend(sampler, c, 200, pool_bytes=80 << 20)
+    _check(c, got, 200)
+    small = _attend(sampler, c, 200)
+    assert (got[0] == small[0]).all() and (got[1] == small[1]).all()
 
 
 def test_no_request_and_empty_table(sampler):
