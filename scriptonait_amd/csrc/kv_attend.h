@@ -325,7 +325,8 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
     begin = 0u;
     end = tiles_of(clamp_len(a.lens[b], most, bad), a.window, E::kTile, first);
   }
-  if (bad && vhead == 0u && (range == 0u || !a.ranges)) atomicOr(a.status, LLMHIP_KSTATUS_BAD_INDEX);
+  // (Any wave may hold the bad length: each lays out a part of a long line.)
+  if (bad && block % teams == 0u && (range == 0u || !a.ranges)) atomicOr(a.status, LLMHIP_KSTATUS_BAD_INDEX);
 
   Run<E, GROUPED, ONCE> run(a);
   run.g = lane >> 4;

@@ -198,6 +198,24 @@ def test_bad_pages_and_lengths_are_left_out(sampler, q, kv, page):
     assert sampler.status().flags == KSTATUS_BAD_INDEX
 
 
+@pytest.mark.parametrize("Hq,spare", [(1, 0), (8, 0), (8, 500)])
+@pytest.mark.parametrize("bad", [0, 63, 64, 70, 299])
+def test_one_bad_length_among_many_is_flagged(sampler, bad, Hq, spare):
+    """Whichever of a workgroup's threads reads it, in ranges and whole."""
+    from scriptonait_amd.kv import KSTATUS_BAD_INDEX
+
+    lens = np.arange(300) % 40
+    lens[bad] = 0
+    c = _make(21, lens, Hq, Hq, 64, 16, "bf16", "bf16", spare=spare)
+    _check(c, _attend(sampler, c))
+    assert sampler.status().flags == 0
+    c["lens"][bad] = -1
+    got = _attend(sampler, c)
+    assert sampler.status().flags == KSTATUS_BAD_INDEX
+    c["lens"][bad] = 0
+    _check(c, got)
+
+
 def test_infinite_scores(sampler):
     """Keys of -inf drop their token, all of them leave a row of zeros."""
     import torch
