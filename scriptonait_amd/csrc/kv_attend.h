@@ -361,8 +361,9 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
     }
   };
 
-  uint32_t tile = begin + (end - begin) * share / a.splits, slot = 2u * wave;
-  const uint32_t stop = begin + (end - begin) * (share + 1u) / a.splits;
+  const uint32_t tiles = end - begin, part = tiles / a.splits, over = tiles - part * a.splits;  // (no product passes 32 bits)
+  uint32_t tile = begin + part * share + over * share / a.splits, slot = 2u * wave;
+  const uint32_t stop = begin + part * (share + 1u) + over * (share + 1u) / a.splits;
   if (a.splits > 1u && lane < 2u) s_slot[slot + lane] = -1;
   if (a.ranges && tile < stop) b = line.at(tile);
   while (tile < stop) {
