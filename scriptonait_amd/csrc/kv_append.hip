@@ -65,7 +65,7 @@ __device__ __forceinline__ void store_once(void* p, const P& x) {
 // A unit's values, rounded, to a row.
 template <class T, int VEC, bool NEIGHBOURS>
 __device__ __forceinline__ void put(typename T::Raw* row, uint32_t d0, uint32_t d1, const float* x) {
-  if constexpr (NEIGHBOURS) {
+  if constexpr (NEIGHBOURS && VEC > 1) {
     Pack<T, 2 * VEC> p;
 #pragma unroll
     for (int j = 0; j < 2 * VEC; ++j) p.v[j] = T::store(x[j]);
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
     const typename X::Raw* row = static_cast<const typename X::Raw*>(a.x[kind]) +
                                  (int64_t)(t0 + t) * a.x_stride[kind][0] + (int64_t)head * a.x_stride[kind][1];
     Pack<X, 2 * VEC> in;
-    if constexpr (NEIGHBOURS) {
+    if constexpr (NEIGHBOURS && VEC > 1) {  // (single values: rows of any alignment)
       in = *reinterpret_cast<const Pack<X, 2 * VEC>*>(row + d0);
     } else {
       const Pack<X, VEC> p0 = *reinterpret_cast<const Pack<X, VEC>*>(row + d0);

@@ -102,6 +102,32 @@ def test_append(sampler, q, kv, T, Hq, Hkv, D, page, dims, style, layout, packed
         assert torch.equal(now[torch.from_numpy(rest)], was.reshape(N * page, -1)[torch.from_numpy(rest)])
 
 
+@pytest.mark.parametrize("style", ["halves", "neighbours"])
+@pytest.mark.parametrize("q,kv", [("f32", "f32"), ("bf16", "bf16"), ("f16", "e4m3")])
+def test_rows_of_any_alignment(sampler, q, kv, style):
+    """Operands that start at an odd value give the bits that aligned ones give."""
+    import torch
+
+    from scriptonait_amd.kv import KVCache, Rope
+
+    X, P = _dtypes(q, kv)
+    T, H, D = 19, 3, 40
+    g = torch.Generator().manual_seed(8)
+    scales = [torch.full((H,), 0.25, device="cuda") for _ in range(2)] if kv == "e4m3" else []
+    x = torch.randn(T, 3 * H, D + 1, generator=g).to(X).cuda()
+    odd = [x[:, i * H:(i + 1) * H, 1:] for i in range(3)]
+    slots, pos = torch.arange(T, device="cuda"), torch.arange(T, dtype=torch.int32, device="cuda") * 37
+    results = []
+    for parts, out in [(odd, torch.zeros(T, H, D + 1, dtype=X, device="cuda")[:, :, 1:]),
+                       ([p.contiguous() for p in odd], torch.zeros(T, H, D, dtype=X, device="cuda"))]:
+        pools = [torch.zeros(2, 16, H, D, device="cuda").to(P) for _ in range(2)]
+        KVCache(sampler, *pools, *scales).append(parts[1], parts[2], slots, q=parts[0], out_q=out, positions=pos,
+                                                 rope=Rope(D, 10000.0, style))
+        results.append([_bytes(t) for t in (out, *pools)])
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and int(results[0][0].count_nonzero()) > 0
+    assert sampler.status().flags == 0
+
+
 def test_in_place_queries_nan_and_bad_slots(sampler):
     import torch
 
