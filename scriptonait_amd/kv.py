@@ -108,25 +108,26 @@ def _table(t, n: int, device):
     return t.data_ptr(), pages, t.stride(0) if n > 1 else pages
 
 
-def _on(stream, tensors) -> int:
+def _on(stream, device, tensors) -> int:
     """A stream of the caller's choice; the tensors' memory is not handed out
     again before it has used them."""
+    if device.type != "cuda":
+        raise ValueError(f"the tensors are on {device}, not on a GPU")
     for t in tensors:
         if t is not None:
             t.record_stream(stream)
     return stream.cuda_stream
 
 
-def _current(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 # torch.cuda.current_stream builds a Stream object for each call (about a
 # microsecond); this is the query beneath it.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-if _raw_stream is not None:
-    def _current(device) -> int:  # noqa: F811
-        return _raw_stream(device.index)
+
+
+def _current(device) -> int:
+    if device.type != "cuda":
+        raise ValueError(f"the tensors are on {device}, not on a GPU")
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
 class Rope:
@@ -185,7 +186,7 @@ class PagePool:
         state moves on; with it ([2] int32) the pool's stays and the new one
         goes there."""
         dev, i32 = self.device, torch.int32
-        R, T = lens.shape[0], slots.shape[0]
+        R, T = lens.numel(), slots.numel()
         state = self.free_state if out_free_state is None else out_free_state
         status = self._plan(
             self.sampler.ctx, self.pages, self.page_size, self._ring, self._state, R, _vector(lens, R, i32, "lens", dev),
@@ -195,8 +196,8 @@ class PagePool:
             _vector(start, R + 1, i32, "start", dev), T, _vector(slots, T, torch.int64, "slots", dev),
             _vector(positions, T, i32, "positions", dev),
             self._state if out_free_state is None else _vector(out_free_state, 2, i32, "out_free_state", dev),
-            _current(dev) if stream is None else _on(stream, (lens, new_tokens, release, table, out_lens, granted, start,
-                                                              slots, positions, state, self.free_ring, self.free_state)))
+            _current(dev) if stream is None else _on(stream, dev, (lens, new_tokens, release, table, out_lens, granted,
+                                                                   start, slots, positions, state, self.free_ring, self.free_state)))
         if status:
             _check(self.lib, status)
 
@@ -251,7 +252,7 @@ class KVCache:
             raise ValueError(f"k is {dt}, which does not go into a {self.dtype} cache")
         if (q is None) != (out_q is None):
             raise ValueError("q and out_q go together")
-        T = k.shape[0]
+        T = slots.numel()
         shape = (T, self.heads, self.head_dim)
         if rope is None:
             turn = None
@@ -271,8 +272,8 @@ class KVCache:
             self.sampler.ctx, self._ref, code, T, *_rows(k, shape, dt, "k", dev), *_rows(v, shape, dt, "v", dev),
             _vector(slots, T, torch.int64, "slots", dev), heads, *q_rows, *out_rows,
             None if positions is None else _vector(positions, T, torch.int32, "positions", dev), turn,
-            _current(dev) if stream is None else _on(stream, (k, v, slots, q, out_q, positions, self.k_pool, self.v_pool,
-                                                              self.k_scale, self.v_scale)))
+            _current(dev) if stream is None else _on(stream, dev, (k, v, slots, q, out_q, positions, self.k_pool,
+                                                                   self.v_pool, self.k_scale, self.v_scale)))
         if status:
             _check(self.lib, status)
 
@@ -315,7 +316,7 @@ class KVCache:
             self.sampler.ctx, self._ref, code, B, heads, *_rows(q, shape, dt, "q", dev), *_table(table, B, dev),
             _vector(lens, B, torch.int32, "lens", dev), window, self._scale if scale is None else scale,
             *_rows(out, shape, dt, "out", dev), lse, _vector(workspace, size, torch.uint8, "workspace", dev), size,
-            _current(dev) if stream is None else _on(stream, (q, table, lens, out, out_lse, workspace, self.k_pool,
-                                                              self.v_pool, self.k_scale, self.v_scale)))
+            _current(dev) if stream is None else _on(stream, dev, (q, table, lens, out, out_lse, workspace, self.k_pool,
+                                                                   self.v_pool, self.k_scale, self.v_scale)))
         if status:
             _check(self.lib, status)

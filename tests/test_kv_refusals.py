@@ -208,3 +208,27 @@ def test_mirror_refuses_wrong_pages_and_ropes():
                         ("new_tokens", i(1)), ("release", i(2).bool()), ("out_free_state", i(1))]:
         with pytest.raises(ValueError):
             pool.plan(**{**args, name: wrong})
+
+
+def test_mirror_refuses_numbers_for_vectors_and_host_memory():
+    """Tensors of no dimension and tensors of the host reach no kernel."""
+    one = torch.zeros((), dtype=torch.int32)
+    c = kv.KVCache(_NoSampler, *_pools())
+    x, slots = torch.zeros(1, 2, 64, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int64)
+    table, lens, ws = torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), torch.zeros(256, dtype=torch.uint8)
+    ring, state = torch.arange(8, dtype=torch.int32), torch.tensor([0, 8], dtype=torch.int32)
+    pool = kv.PagePool(_NoSampler, 8, 16, ring, state)
+    rest = (lens.clone(), lens.clone(), torch.zeros(2, dtype=torch.int32))
+    for bad in [lambda: c.append(one.bfloat16(), x, slots), lambda: c.append(x, x, one.long()),
+                lambda: c.append(x, x, slots, q=one.bfloat16(), out_q=one.bfloat16()),
+                lambda: c.attend(one.bfloat16(), table, lens, x, ws), lambda: c.attend(x, one, lens, x, ws),
+                lambda: c.attend(x, table, one, x, ws), lambda: pool.plan(one, table, *rest, slots, lens),
+                lambda: pool.plan(lens, table, *rest, one.long(), lens)]:
+        with pytest.raises(ValueError):
+            bad()
+    for bad in [lambda: c.append(x, x, slots), lambda: c.attend(x, table, lens, x.clone(), ws),
+                lambda: pool.plan(lens, table, *rest, slots, lens.clone()),
+                lambda: c.append(x, x, slots, stream=object()), lambda: c.attend(x, table, lens, x.clone(), ws, stream=object()),
+                lambda: pool.plan(lens, table, *rest, slots, lens.clone(), stream=object())]:
+        with pytest.raises(ValueError, match="not on a GPU"):
+            bad()
