@@ -98,16 +98,19 @@ typedef struct llmhip_rope {
  *                 first that the free pages do not reach for, every request
  *                 that needs a page is refused in this call
  *   start         device [R + 1] each request's first token in the batch
- *                 (refused requests keep their gap) and their sum
+ *                 (refused requests keep their gap) and their sum, at most
+ *                 2^31 - 1
  *   slots         device [T] each token's slot; -1 in gaps and past the end
  *   positions     device [T] each token's position; 0 there
  *   out_free_state device [2] the pool's state after the call (may be
  *                 free_state). ring and table change in place
  *
  * A length outside [0, table_pages * page], a negative new_tokens, a free
- * state outside the ring and a page id outside the pool set
+ * state outside the ring and a page id outside the pool (a released one
+ * too, which goes back as it is) set
  * LLMHIP_KSTATUS_BAD_INDEX: the length is clamped, the count taken as 0, the
- * pool as empty, and the token's slot is -1.
+ * pool as empty, and the token's slot is -1. Apart from out_lens and
+ * out_free_state no output may overlap an input.
  */
 int llmhip_kv_plan(llmhip_ctx* ctx, size_t pages, size_t page, int32_t* ring, const int32_t* free_state, size_t R,
                    const int32_t* lens, const int32_t* new_tokens, const int32_t* release, int32_t* table,

@@ -38,11 +38,12 @@ int launched(hipError_t e, const char* what) {
 #define SUPPORTED(cond, what) \
   if (!(cond)) return unsupported(what)
 
-// Two arrays of n values are one and the same, or apart.
-bool same_or_apart(const int32_t* x, const int32_t* y, size_t n) {
+// An array of n values and one of m share no memory; a null one shares none.
+bool apart(const int32_t* x, size_t n, const int32_t* y, size_t m) {
   const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
-  return a == b || a + n * sizeof(int32_t) <= b || b + n * sizeof(int32_t) <= a;
+  return !x || !y || a + n * sizeof(int32_t) <= b || b + m * sizeof(int32_t) <= a;
 }
+bool same_or_apart(const int32_t* x, const int32_t* y, size_t n) { return x == y || apart(x, n, y, n); }
 
 constexpr size_t kMaxInt = 0x7fffffff;
 constexpr size_t kMaxBatch = 65535;
@@ -144,6 +145,11 @@ int llmhip_kv_plan(llmhip_ctx* ctx, size_t pages, size_t page, int32_t* ring, co
   ARG(same_or_apart(lens, out_lens, R), "lens and out_lens overlap");
   ARG(same_or_apart(free_state, out_free_state, 2), "free_state and out_free_state overlap");
   ON_DEVICE(info);
+  // Workgroups read what each request asks for while others write the results.
+  for (const int32_t* in : {lens, new_tokens, release}) {
+    ARG(apart(in, R, granted, R) && apart(in, R, start, R + 1), "granted and start must not overlap what they follow from");
+    ARG(in == lens || apart(in, R, out_lens, R), "out_lens overlaps new_tokens or release");
+  }
   PlanArgs a{};
   a.ring = ring;
   a.free_state = free_state;

@@ -126,7 +126,7 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
     if (sums && r < a.R) {
       a.out_lens[r] = (int32_t)(base + (ok ? (uint32_t)n : 0u));
       a.granted[r] = ok ? (int32_t)n : 0;
-      a.start[r + 1u] = (int32_t)(uint32_t)end;
+      a.start[r + 1u] = (int32_t)min(end, (uint64_t)0x7fffffffu);
     }
     __syncthreads();
 
@@ -137,7 +137,11 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(PlanArgs a) {
         const uint32_t back_i = s_back[i], fresh = back_i ? s_took[i] : 0u;
         int32_t* row = a.table + (uint64_t)(r0 + i) * a.table_ld;
         for (uint32_t p = tid & 63u; p < max(back_i, fresh); p += 64u) {
-          if (p < back_i) a.ring[in_ring((uint64_t)s_put[i] + p, a.pages)] = row[p];
+          if (p < back_i) {
+            const int32_t id = row[p];
+            bad = bad || (uint32_t)id >= a.pages;
+            a.ring[in_ring((uint64_t)s_put[i] + p, a.pages)] = id;
+          }
           if (p < fresh) row[p] = a.ring[in_ring((uint64_t)s_first[i] + p, a.pages)];
         }
       }

@@ -117,6 +117,49 @@ def test_bad_values_are_flagged_and_followed_nowhere(sampler, change):
     assert 0 <= got["state"][0] < 4 and 0 <= got["state"][1] <= 4
 
 
+def test_sums_past_31_bits_stop_there(sampler):
+    most = 2**31 - 1
+    c = dict(page=4, ring=[3, 2, 1, 0], state=[0, 4], lens=[0, 0, 0, 0], table=[[-7, -7]] * 4, T=6, new=[2, most, most, 1])
+    got = _run(sampler, **c)
+    assert got["start"] == [0, 2, most, most, most] and got["granted"] == [2, 0, 0, 0]
+    assert got["slots"] == [12, 13, -1, -1, -1, -1] and got["state"] == [1, 3]
+    assert sampler.status().flags == 0
+
+
+def test_released_pages_outside_the_pool_are_flagged(sampler):
+    from scriptonait_amd.kv import KSTATUS_BAD_INDEX
+
+    c = dict(page=4, ring=[3, 2, 1, 0], state=[0, 1], lens=[8, 3], table=[[1, 4], [0, -7]], T=2, release=[1, 0])
+    sampler.status()
+    got = _run(sampler, **c)
+    assert sampler.status().flags == KSTATUS_BAD_INDEX
+    assert got["ring"][1:3] == [1, 4] and got["state"] == [0, 3] and got["slots"] == [3, -1]
+    c["table"] = [[1, 2], [0, -7]]
+    _run(sampler, **c)
+    assert sampler.status().flags == 0
+
+
+def test_outputs_over_inputs_are_refused(sampler):
+    import torch
+
+    from scriptonait_amd.kv import PagePool
+    from scriptonait_amd.sampler import SamplerError
+
+    x = torch.zeros(64, dtype=torch.int32, device="cuda")
+    pool = PagePool(sampler, 8, 16)
+    table = torch.zeros(4, 2, dtype=torch.int32, device="cuda")
+    slots = torch.zeros(4, dtype=torch.int64, device="cuda")
+    args = dict(lens=x[:4], out_lens=x[4:8], granted=x[8:12], start=x[12:17], slots=slots, positions=x[20:24],
+                new_tokens=x[24:28], release=x[28:32], table=table)
+    for change in [dict(granted=x[24:28]), dict(granted=x[2:6]), dict(start=x[28:33]), dict(start=x[20:25], lens=x[24:28]),
+                   dict(out_lens=x[31:35]), dict(out_lens=x[3:7]), dict(out_lens=x[24:28])]:
+        with pytest.raises(SamplerError, match="overlap"):
+            pool.plan(**{**args, **change})
+    pool.plan(**args)
+    pool.plan(**{**args, "out_lens": args["lens"]})
+    assert sampler.status().flags == 0
+
+
 def test_other_stream(sampler):
     import torch
 
