@@ -125,9 +125,12 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _current(device) -> int:
-    if device.type != "cuda":
-        raise ValueError(f"the tensors are on {device}, not on a GPU")
-    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+    try:
+        return _raw_stream(device.index)
+    except (TypeError, RuntimeError):  # no such query, or the host's device, which has no index
+        if device.type != "cuda":
+            raise ValueError(f"the tensors are on {device}, not on a GPU") from None
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 class Rope:
