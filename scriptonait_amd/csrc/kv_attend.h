@@ -6,7 +6,8 @@
 // runs are joined by l = sum_k l_k 2^(m_k - M), o likewise, and the answer
 // is o / l. m moves only when a score passes it by more than 8: the
 // numerators then stay below 2^8 and the largest is at least 1, and most
-// tiles neither compare across lanes nor scale o.
+// tiles neither compare across lanes nor scale o. (Where they are held as F16
+// m is 7 lower, for their small ones: 2^15, and at least 2^7.)
 //
 // The work is every request's tiles of tokens in one line, cut into equal
 // ranges, so ragged lengths share the card evenly and one long request uses
@@ -130,7 +131,7 @@ struct Run {
   uint32_t g, c, lo, hi;  // the lane, and the tokens that are seen
   float scale;            // of a score, in base-2 exponents
   E e;
-  float ref, limit, sum;  // m (0 before the first finite score), m + 8, the lane's part of l
+  float ref, limit, sum;  // m (0 before the first finite score), what no score passes, the lane's part of l
   bool bad = false;
   struct Ids {
     uint32_t k[kKIds], v[kIds];
@@ -265,11 +266,12 @@ struct Run {
   __device__ __forceinline__ void raise(float top) {
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const bool fresh = limit == -INFINITY, up = top > (fresh ? -INFINITY : ref);
-    const float next = up ? top : ref;
+    const float low = top - E::kLift;
+    const bool fresh = limit == -INFINITY, up = low > (fresh ? -INFINITY : ref);
+    const float next = up ? low : ref;
     const float keep = fresh || !up ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
     ref = next;
-    limit = up || !fresh ? next + kLazyBits : -INFINITY;
+    limit = up || !fresh ? next + (E::kLift + kLazyBits) : -INFINITY;
     sum *= keep;
     f32x4 k;
 #pragma unroll

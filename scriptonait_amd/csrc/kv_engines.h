@@ -19,6 +19,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "kv_types.h"
 
 namespace llmhip {
@@ -111,6 +113,14 @@ struct Engine16 {
   // 8: no load or store passes the row's end.
   static constexpr int kVec = DIM == 32 ? 2 : DIM == 64 || (DIM == 192 && kElem == 2) ? 4 : 8;
   static constexpr int kPanels = (DIM + 16 * kVec - 1) / (16 * kVec);
+  // The numerators' and values' type in the second product. E4M3 values are
+  // exact in either; BF16 numerators have no smallest step to lose.
+  using W = std::conditional_t<std::is_same_v<KV, E4M3>, BF16, Q>;
+  // F16 has: numerators are held 2^kLift times as large, up to 2^15, and what
+  // their rounding lost kSpread times as large again.
+  static constexpr bool kNarrow = std::is_same_v<W, F16>;
+  static constexpr float kLift = kNarrow ? 7.0f : 0.0f;
+  static constexpr float kSpread = 4096.0f;
   using KRaw = typename RawOf<CHUNK * kElem>::type;
   using VRaw = typename RawOf<kVec * kElem>::type;
 
@@ -184,7 +194,10 @@ struct Engine16 {
           } else {
             y = k[a][t];
           }
-          if (!FULL) y &= keep;
+          if constexpr (!FULL) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] &= keep;
+          }
           x = mfma(Q(), y, q[t][h], x);
         }
       }
@@ -205,21 +218,39 @@ struct Engine16 {
     uint32_t x;
     if constexpr (kVec * kElem <= 4) x = v[i][p];
     else x = v[i][p][kElem == 1 ? w >> 1 : w];
-    if constexpr (kElem == 1) return w & 1 ? widen2<true>(Q(), x) : widen2<false>(Q(), x);
+    if constexpr (kElem == 1) return w & 1 ? widen2<true>(W(), x) : widen2<false>(W(), x);
     else return x;
+  }
+
+  __device__ __forceinline__ static void add_product(u32x4 hi, u32x4 lo, u32x4 v, f32x4& x) {
+    if constexpr (kNarrow) {
+      const f32x4 y = mfma(W(), lo, v, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(y[i], 1.0f / kSpread, x[i]);
+    } else {
+      x = mfma(W(), lo, v, x);
+    }
+    x = mfma(W(), hi, v, x);
   }
 
   // O += P V. A numerator is held as the sum of two 16-bit values, the
   // second what the first one's rounding lost: the matrix cores have the time
-  // (24 products for 16 KiB of cache), and 16 bits of it are kept, not 8.
+  // (24 products for 16 KiB of cache), and at least 16 bits of it are kept, not 8.
+  // BF16 loses 2^-17 of a numerator. F16 loses 2^-23 of it or, as its smallest
+  // step is 2^-24, 2^-25 in the second value's scale: 2^-44 of the largest
+  // numerator, which is at least 2^kLift. So n tokens are off by at most
+  // n 2^-44 max |v|; values without a scale, of a sum that has all
+  // numerators, were off by n 2^-25 max |v|.
   __device__ __forceinline__ void accumulate(const float* s) {
     u32x4 hi, lo;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      hi[i] = pack2(Q(), s[2 * i], s[2 * i + 1]);
+      hi[i] = pack2(W(), s[2 * i], s[2 * i + 1]);
       float x, y;
-      unpack2(Q(), hi[i], x, y);
-      lo[i] = pack2(Q(), s[2 * i] - x, s[2 * i + 1] - y);
+      unpack2(W(), hi[i], x, y);
+      x = s[2 * i] - x;
+      y = s[2 * i + 1] - y;
+      lo[i] = kNarrow ? pack2(W(), x * kSpread, y * kSpread) : pack2(W(), x, y);
     }
 #pragma unroll
     for (int p = 0; p < kPanels; ++p) {
@@ -232,10 +263,8 @@ struct Engine16 {
           even[i] = __builtin_amdgcn_perm(y, x, 0x05040100u);
           odd[i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
         }
-        o[p][2 * w] = mfma(Q(), lo, even, o[p][2 * w]);
-        o[p][2 * w + 1] = mfma(Q(), lo, odd, o[p][2 * w + 1]);
-        o[p][2 * w] = mfma(Q(), hi, even, o[p][2 * w]);
-        o[p][2 * w + 1] = mfma(Q(), hi, odd, o[p][2 * w + 1]);
+        add_product(hi, lo, even, o[p][2 * w]);
+        add_product(hi, lo, odd, o[p][2 * w + 1]);
       }
     }
   }
@@ -251,6 +280,7 @@ struct Engine32 {
   static constexpr int kDim = DIM;
   static constexpr int kGroup = 4, kTile = 16, kProducts = 1;
   static constexpr int kSteps = DIM / 16;
+  static constexpr float kLift = 0.0f;
   static constexpr int kVec = DIM % 64 ? 2 : 4, kPanels = DIM / (16 * kVec);
   using VRaw = float __attribute__((ext_vector_type(kVec)));
 
