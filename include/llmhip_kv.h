@@ -172,7 +172,8 @@ int llmhip_kv_attend_workspace(llmhip_ctx* ctx, const llmhip_kv_cache* cache, si
  * and logarithms are the hardware's to base 2. With 16-bit queries each
  * softmax weight meets the values as the sum of two 16-bit numbers: off by at
  * most 2^-17 of itself, or in an F16 cache by 2^-23 of itself or 2^-44 of the
- * largest weight.
+ * largest weight. An infinite value that a token of a weight above 0 holds
+ * makes its column infinite, or NaN beside one of the other sign.
  */
 int llmhip_kv_attend(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dtype, size_t B, size_t q_heads,
                      const void* q, int64_t q_request, int64_t q_head, const int32_t* table, size_t table_pages,

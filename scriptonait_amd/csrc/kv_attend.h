@@ -131,8 +131,9 @@ struct Run {
   uint32_t g, c, lo, hi;  // the lane, and the tokens that are seen
   float scale;            // of a score, in base-2 exponents
   E e;
-  float ref, limit, sum;  // m (0 before the first finite score), what no score passes, the lane's part of l
+  float ref, limit, sum = 0.0f;  // m (0 before the first finite score), what no score passes, the lane's part of l
   bool bad = false;
+  enum { kAllValues, kFinite, kInfinite } values = kAllValues;  // which ones a pass adds
   struct Ids {
     uint32_t k[kKIds], v[kIds];
   };
@@ -208,10 +209,13 @@ struct Run {
   // load. The last tile loads itself again (from the L2): a branch around the
   // loads would make every wait one for all of them.
   __device__ __forceinline__ void tiles(uint32_t first, uint32_t last) {
-    ref = 0.0f;
-    limit = -INFINITY;
-    sum = 0.0f;
-    e.clear();
+    const float before = sum;
+    if (!E::kInfinities || values != kInfinite) {
+      ref = 0.0f;
+      limit = -INFINITY;
+      sum = 0.0f;
+      e.clear();
+    }
     uint32_t t0 = readlane_u32(first, 0) * E::kTile;  // (the same in every lane: the loop's branch is the wave's)
     const uint32_t t_last = (readlane_u32(last, 0) - 1u) * E::kTile;
     const Ids now = fetch_ids(t0);
@@ -233,11 +237,25 @@ struct Run {
       next = after;
       t0 = t1;
     } while (more);
+    if (E::kInfinities && values == kInfinite) sum = before;
+  }
+
+  // Whether the tiles have to be read again, for sums that are not finite: a
+  // second pass adds the finite values alone, a third the others, which their
+  // signs decide.
+  __device__ __forceinline__ bool again() {
+    if constexpr (E::kInfinities) {
+      if (__builtin_expect(values != kAllValues || __any(e.infinite()), 0)) {
+        values = values == kAllValues ? kFinite : values == kFinite ? kInfinite : kAllValues;
+        return values != kAllValues;
+      }
+    }
+    return false;
   }
 
   // A tile's scores and values into ref, sum and o.
   __device__ __forceinline__ void add(float* s, uint32_t seen) {
-    const bool edge = __any(seen != kAll);
+    const bool edge = __any(seen != kAll) || (E::kInfinities && values != kAllValues);
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < E::kGroup; ++i) {
@@ -255,6 +273,16 @@ struct Run {
         const bool keep = seen >> i & 1u;
         s[i] = keep ? s[i] : 0.0f;
         e.keep_v(i, keep);
+      }
+      if constexpr (E::kInfinities) {
+        if (__builtin_expect(values != kAllValues, 0)) {
+#pragma unroll
+          for (int i = 0; i < E::kGroup; ++i) {
+            // A numerator above 0 whose two parts are.
+            if (values == kInfinite) s[i] = s[i] > 0.0f ? 1.0f + 0x1p-12f : s[i];
+            e.keep_finite(i, values == kFinite);
+          }
+        }
       }
     }
 #pragma unroll
@@ -387,6 +415,7 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
                                   (int64_t)(qhead + (run.c < group ? run.c : 0u)) * a.q_stride[1];
     run.e.load_q(q, run.g, a.dim, run.c < group);
     run.tiles(zero_tile + (tile - from), zero_tile + (last - from));
+    if (run.again()) continue;
     const float l = run.total(), m = l == 0.0f ? -INFINITY : run.ref;
     if (tile == from && last == to) {  // all of the request
       const float inv = l == 0.0f ? 0.0f : vscale / l;
@@ -455,14 +484,15 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
   uint64_t rest = __ballot(holds >= 0);
   while (rest) {
     const uint32_t r = readlane_u32((uint32_t)holds, (uint32_t)__builtin_ctzll(rest));
-    uint64_t set = __ballot(holds == (int32_t)r);
-    rest &= ~set;
-    const uint32_t n = (uint32_t)__builtin_popcountll(set);
+    const uint64_t parts = __ballot(holds == (int32_t)r);
+    rest &= ~parts;
+    const auto part_at = [&](uint32_t i) { return s_part + (2u * ((i >> 1) * a.team + mate) + (i & 1u)) * a.part_words; };
+    const uint32_t n = (uint32_t)__builtin_popcountll(parts);
+    uint64_t set = parts;
     const float* part[kWaves];
 #pragma unroll
     for (uint32_t k = 0; k < kWaves; ++k) {
-      const uint32_t i = (uint32_t)__builtin_ctzll(set);
-      part[k] = k < n ? s_part + (2u * ((i >> 1) * a.team + mate) + (i & 1u)) * a.part_words : part[0];
+      part[k] = k < n ? part_at((uint32_t)__builtin_ctzll(set)) : part[0];
       set &= set - 1u;
     }
     const bool before = a.ranges && line.start(r) < begin, after = a.ranges && line.end(r) > end;
@@ -481,6 +511,13 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
         w[k] = __builtin_amdgcn_exp2f(w[k] - top);
         l += part[k][at_l] * w[k];
         o += part[k][x] * w[k];
+      }
+      if (__builtin_expect(!isfinite(o), 0)) {  // without the missing parts: 0 times an infinite sum is NaN
+        o = 0.0f;
+        for (uint64_t left = parts; left; left &= left - 1u) {
+          const float* p = part_at((uint32_t)__builtin_ctzll(left));
+          o += p[x] * __builtin_amdgcn_exp2f(p[at_m] - top);
+        }
       }
       if (before || after) {
         to[x] = o;
@@ -523,6 +560,9 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
   const uint32_t head = qh / a.group, in_group = qh % a.group, vhead = head * a.blocks + in_group / 16u;
   const uint32_t group = min(16u, a.group - in_group / 16u * 16u), qi = in_group % 16u;
   const uint32_t at_o = qi * a.dim + d, at_m = group * a.dim + qi, at_l = at_m + group;
+  const auto part_at = [&](uint32_t k) {
+    return a.workspace + a.part_offset + (((uint64_t)(cut.first + k) * a.vheads + vhead) * 2u + (k ? 0u : 1u)) * a.part_words;
+  };
   float m = -INFINITY, l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   for (uint32_t k0 = share; k0 < n; k0 += kBatch * shares) {
@@ -531,8 +571,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
 #pragma unroll
     for (uint32_t j = 0; j < kBatch; ++j) {  // (the first one again where there is no more)
       const uint32_t k = k0 + j * shares < n ? k0 + j * shares : k0;
-      const float* part =
-          a.workspace + a.part_offset + (((uint64_t)(cut.first + k) * a.vheads + vhead) * 2u + (k ? 0u : 1u)) * a.part_words;
+      const float* part = part_at(k);
       pm[j] = part[at_m];
       pl[j] = part[at_l];
       po[j] = *reinterpret_cast<const f32x4*>(part + at_o);
@@ -553,6 +592,13 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
       o += po[j] * w;
     }
     m = next;
+  }
+  if (__builtin_expect(!isfinite((o[0] + o[1]) + (o[2] + o[3])), 0)) {  // without the missing parts: 0 times an infinite sum is NaN
+    o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t k = share; k < n; k += shares) {
+      const float* part = part_at(k);
+      o += *reinterpret_cast<const f32x4*>(part + at_o) * __builtin_amdgcn_exp2f(part[at_m] - (m == -INFINITY ? 0.0f : m));
+    }
   }
   if (shares > 1u) {
     s_m[tid] = m;

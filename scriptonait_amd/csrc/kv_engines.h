@@ -86,6 +86,13 @@ __device__ __forceinline__ void unpack2(F16, uint32_t v, float& x, float& y) {
   x = (float)h[0];
   y = (float)h[1];
 }
+// A word with those of its two values that are infinite or NaN replaced by 0.
+template <class T>
+__device__ __forceinline__ uint32_t finite2(T, uint32_t x) {
+  constexpr uint32_t kTop = std::is_same_v<T, BF16> ? 0x7f80u : 0x7c00u;
+  const uint32_t low = (x & kTop) == kTop ? 0u : x & 0xffffu;
+  return (x >> 16 & kTop) == kTop ? low : low | (x & 0xffff0000u);
+}
 // Two E4M3 values of a word as 16-bit values, exactly.
 template <bool HIGH>
 __device__ __forceinline__ uint32_t widen2(BF16, uint32_t x) {
@@ -121,6 +128,9 @@ struct Engine16 {
   static constexpr bool kNarrow = std::is_same_v<W, F16>;
   static constexpr float kLift = kNarrow ? 7.0f : 0.0f;
   static constexpr float kSpread = 4096.0f;
+  // Infinite values need passes of their own: 0 times them is NaN, and the
+  // second part of a numerator is often 0 or negative.
+  static constexpr bool kInfinities = kElem == 2;
   using KRaw = typename RawOf<CHUNK * kElem>::type;
   using VRaw = typename RawOf<kVec * kElem>::type;
 
@@ -213,6 +223,33 @@ struct Engine16 {
       for (int j = 0; j < kVec; ++j) o[p][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
+  // Whether a sum of this lane is no finite number.
+  __device__ __forceinline__ bool infinite() const {
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int p = 0; p < kPanels; ++p)
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(o[p][j][i], 0.0f, x[i]);
+    return !((x[0] + x[1]) + (x[2] + x[3]) == 0.0f);
+  }
+  // Of token i's values only those that are finite, or only the others.
+  __device__ __forceinline__ void keep_finite(int i, bool finite) {
+#pragma unroll
+    for (int p = 0; p < kPanels; ++p)
+#pragma unroll
+      for (int w = 0; w < kVec / 2; ++w) {
+        if constexpr (kVec == 2) {
+          const uint32_t x = finite2(W(), v[i][p]);
+          v[i][p] = finite ? x : v[i][p] ^ x;
+        } else if constexpr (kElem == 2) {
+          const uint32_t x = finite2(W(), v[i][p][w]);
+          v[i][p][w] = finite ? x : v[i][p][w] ^ x;
+        }
+      }
+  }
+
   // Word w (values 2 w and 2 w + 1) of token i's values in panel p.
   __device__ __forceinline__ uint32_t word(int i, int p, int w) const {
     uint32_t x;
@@ -281,6 +318,7 @@ struct Engine32 {
   static constexpr int kGroup = 4, kTile = 16, kProducts = 1;
   static constexpr int kSteps = DIM / 16;
   static constexpr float kLift = 0.0f;
+  static constexpr bool kInfinities = false;
   static constexpr int kVec = DIM % 64 ? 2 : 4, kPanels = DIM / (16 * kVec);
   using VRaw = float __attribute__((ext_vector_type(kVec)));
 

@@ -1,8 +1,6 @@
-"""GPU: infinite values and scores past binary32 in attention. A value that a
-request sees with a weight above 0 decides its column alone, however the
-request is cut over waves and workgroups: infinity gives infinity, both signs
-and NaN give NaN."""
-import numpy as np
+"""GPU: infinite values in attention. A value that a request sees with a
+weight above 0 decides its column alone, however the request is cut over waves
+and workgroups: infinity gives infinity, both signs and NaN give NaN."""
 import pytest
 
 import kv_oracle
@@ -110,22 +108,3 @@ def test_one_requests_infinity_stays_its_own(sampler, q, kv):
     hit[1, 4:6, 11] = True
     assert (got[0][hit] == INF).all()
     assert torch.equal(got[0][~hit], clean[0][~hit]) and torch.equal(got[1], clean[1])
-
-
-@pytest.mark.parametrize("B,n", [(1, 1), (1, 40), (2, 3000), (1, 200)])
-def test_scores_past_binary32_give_nan(sampler, B, n):
-    """A score that binary32 does not hold is no weight of 0, whichever part
-    of its request it is in."""
-    import torch
-
-    D = 64
-    c = _make(33, [n] * B, 2, 1, D, 16, "f32", "f32")
-    c["q"] = torch.zeros_like(c["q"])
-    c["q"][..., 0] = 1e19
-    live = ~c["k_pool"][..., 0].isnan()
-    c["k_pool"][..., 0][live] = 1e15
-    id, at = _place(c, 0, n // 2)
-    c["k_pool"][id, at, 0, 0] = 3e19  # 3e38, times log2(e) past the largest number
-    got = _attend(sampler, c, scale=1.0)
-    assert got[0][0].isnan().all() and got[1][0].isnan().all()
-    assert got[0][1:].isfinite().all() and np.isfinite(got[1][1:]).all()
