@@ -169,7 +169,8 @@ int llmhip_kv_attend_workspace(llmhip_ctx* ctx, const llmhip_kv_cache* cache, si
  * A length outside [0, table_pages * page] is clamped, and tokens on a page
  * id outside the pool are left out; both are flagged.
  * Scores, maxima, sums and outputs are accumulated in binary32, exponentials
- * and logarithms are the hardware's to base 2. With 16-bit queries each
+ * and logarithms are the hardware's to base 2; a score that times log2(e)
+ * passes binary32's largest number gives a row of NaN. With 16-bit queries each
  * softmax weight meets the values as the sum of two 16-bit numbers: off by at
  * most 2^-17 of itself, or in an F16 cache by 2^-23 of itself or 2^-44 of the
  * largest weight. An infinite value that a token of a weight above 0 holds

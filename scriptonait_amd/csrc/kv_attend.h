@@ -132,6 +132,7 @@ struct Run {
   float scale;            // of a score, in base-2 exponents
   E e;
   float ref, limit, sum = 0.0f;  // m (0 before the first finite score), what no score passes, the lane's part of l
+  bool far = false;  // some |m| is 2^20 or more
   bool bad = false;
   enum { kAllValues, kFinite, kInfinite } values = kAllValues;  // which ones a pass adds
   struct Ids {
@@ -212,6 +213,7 @@ struct Run {
     const float before = sum;
     if (!E::kInfinities || values != kInfinite) {
       ref = 0.0f;
+      far = false;
       limit = -INFINITY;
       sum = 0.0f;
       e.clear();
@@ -264,9 +266,23 @@ struct Run {
     }
     if (__any(top > limit)) raise(top);
     // The scaled score is not rounded before the reference is taken from it:
-    // only the difference is, and that is small where it counts.
+    // only the difference is, and that is small where it counts. The reference
+    // is a rounded one, so the largest difference is as far from 0 as half of
+    // its last bit: far references take the rounded scores' difference, which
+    // is exact there.
+    if (__builtin_expect(far, 0)) {
 #pragma unroll
-    for (int i = 0; i < E::kGroup; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -ref));
+      for (int i = 0; i < E::kGroup; ++i) {
+        s[i] = s[i] * scale - ref;
+        // (The limit is rounded too: by a last bit of 16 to past the largest F16.)
+        if (E::kLift > 0.0f) s[i] = s[i] > E::kLift + kLazyBits ? E::kLift + kLazyBits : s[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E::kGroup; ++i) s[i] = __builtin_fmaf(s[i], scale, -ref);
+    }
+#pragma unroll
+    for (int i = 0; i < E::kGroup; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]);
     if (edge) {
 #pragma unroll
       for (int i = 0; i < E::kGroup; ++i) {
@@ -298,7 +314,8 @@ struct Run {
     const bool fresh = limit == -INFINITY, up = low > (fresh ? -INFINITY : ref);
     const float next = up ? low : ref;
     const float keep = fresh || !up ? 1.0f : __builtin_amdgcn_exp2f(ref - next);
-    ref = next;
+    ref = next == INFINITY ? NAN : next;  // (past binary32: no weight of 0, but NaN)
+    far = __any(fabsf(ref) >= 0x1p20f);
     limit = up || !fresh ? next + (E::kLift + kLazyBits) : -INFINITY;
     sum *= keep;
     f32x4 k;
