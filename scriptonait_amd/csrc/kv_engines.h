@@ -51,9 +51,11 @@ template <>
 struct RawOf<16> { using type = u32x4; };
 
 // Keys: two neighbouring loads share a cache line, the first level keeps it.
-template <class T>
+// ALIGN: what the rows are aligned to, which E4M3's are to 8 bytes.
+template <class T, int ALIGN = sizeof(T)>
 __device__ __forceinline__ T load_key(const char* p) {
-  return *reinterpret_cast<const T*>(p);
+  typedef T __attribute__((aligned(ALIGN))) Placed;
+  return *reinterpret_cast<const Placed*>(p);
 }
 // Values: whole lines; ONCE: past the caches' reach before they are read again.
 template <class T, bool ONCE>
@@ -167,7 +169,7 @@ struct Engine16 {
     for (uint32_t s = 0; s < kLoads; ++s) {
       uint32_t d;
       chunk(s, g, dim, d);
-      k[a][s] = load_key<KRaw>(row + d * kElem);
+      k[a][s] = load_key<KRaw, kElem == 1 ? 8 : sizeof(KRaw)>(row + d * kElem);
     }
   }
 
