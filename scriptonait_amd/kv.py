@@ -113,6 +113,8 @@ def _on(stream, device, tensors) -> int:
     again before it has used them."""
     if device.type != "cuda":
         raise ValueError(f"the tensors are on {device}, not on a GPU")
+    if getattr(stream, "device", device) != device:
+        raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
     for t in tensors:
         if t is not None:
             t.record_stream(stream)
@@ -131,6 +133,14 @@ def _current(device) -> int:
         if device.type != "cuda":
             raise ValueError(f"the tensors are on {device}, not on a GPU") from None
         return torch.cuda.current_stream(device).cuda_stream
+
+
+def _same_gpu(sampler: Sampler, device) -> None:
+    """Kernels and flags are the sampler's device's. (The host's tensors are
+    refused where a call would use them.)"""
+    index = getattr(sampler, "device", device.index)
+    if device.type == "cuda" and device.index != index:
+        raise ValueError(f"the tensors are on {device}, the sampler on cuda:{index}")
 
 
 class Rope:
@@ -161,8 +171,8 @@ class PagePool:
     """The free pages of a pool of `pages` pages of `page_size` tokens.
     free_ring ([pages] int32) and free_state ([2] int32: the first free id's
     place in the ring, and how many are free) live on the device; without
-    them every page starts out free. One pool's plan serves the caches of all
-    layers, whose page ids are the same."""
+    them every page starts out free, on the sampler's device. One pool's plan
+    serves the caches of all layers, whose page ids are the same."""
 
     def __init__(self, sampler: Sampler, pages: int, page_size: int, free_ring=None, free_state=None, device=None):
         if pages < 1 or page_size < 1:
@@ -170,11 +180,12 @@ class PagePool:
         if (free_ring is None) != (free_state is None):
             raise ValueError("free_ring and free_state go together")
         if free_ring is None:
-            device = torch.device("cuda:0") if device is None else torch.device(device)
+            device = torch.device("cuda", sampler.device) if device is None else torch.device(device)
             free_ring = torch.arange(pages, dtype=torch.int32, device=device)
             free_state = torch.tensor([0, pages], dtype=torch.int32, device=device)
         self.sampler, self.lib, self.pages, self.page_size = sampler, load_kv(), pages, page_size
         self.device = free_ring.device
+        _same_gpu(sampler, self.device)
         self._ring = _vector(free_ring, pages, torch.int32, "free_ring", self.device)
         self._state = _vector(free_state, 2, torch.int32, "free_state", self.device)
         self.free_ring, self.free_state = free_ring, free_state
@@ -227,6 +238,7 @@ class KVCache:
         if dim % 8 or not 8 <= dim <= 256:
             raise ValueError("head_dim must be a multiple of 8 up to 256")
         self.dtype, self.device = k_pool.dtype, k_pool.device
+        _same_gpu(sampler, self.device)
         if (self.dtype == torch.float8_e4m3fn) != (k_scale is not None) or (k_scale is None) != (v_scale is None):
             raise ValueError("k_scale and v_scale go with float8_e4m3fn pools, and only with those")
         self.sampler, self.lib = sampler, load_kv()

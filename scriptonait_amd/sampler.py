@@ -216,6 +216,7 @@ class Sampler:
         ctx = ctypes.c_void_p()
         _check(self.lib, self.lib.llmhip_ctx_create(device, ctypes.byref(ctx)))
         self.ctx = ctx
+        self.device = device
 
     def close(self) -> None:
         if self.ctx:
