@@ -136,7 +136,8 @@ int llmhip_kv_plan(llmhip_ctx* ctx, size_t pages, size_t page, int32_t* ring, co
  *
  * Values are rotated in binary32 and rounded once to the output's type, to
  * nearest even; an E4M3 cache takes value / scale[head], clamped to +-448.
- * A slot past the pool is skipped and flagged.
+ * A slot past the pool is skipped and flagged. Rows of a pool or of out_q that
+ * overlap (strides below head_dim) are refused.
  */
 int llmhip_kv_append(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dtype, size_t T, const void* k,
                      int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
@@ -167,7 +168,8 @@ int llmhip_kv_attend_workspace(llmhip_ctx* ctx, const llmhip_kv_cache* cache, si
  *              the call. Calls that overlap need one each
  *
  * A length outside [0, table_pages * page] is clamped, and tokens on a page
- * id outside the pool are left out; both are flagged.
+ * id outside the pool are left out; both are flagged. Rows of out that overlap
+ * are refused.
  * Scores, maxima, sums and outputs are accumulated in binary32, exponentials
  * and logarithms are the hardware's to base 2; a score that times log2(e)
  * passes binary32's largest number gives a row of NaN. With 16-bit queries each

@@ -59,6 +59,13 @@ bool rows_on(const void* p, const int64_t* strides, int n, uint32_t elem, uint32
   return true;
 }
 
+// Whether neighbours in each direction have `dim` values to themselves.
+bool rows_apart(const int64_t* strides, const uint64_t* extents, int n, uint32_t dim) {
+  for (int i = 0; i < n; ++i)
+    if (extents[i] > 1 && strides[i] < (int64_t)dim && strides[i] > -(int64_t)dim) return false;
+  return true;
+}
+
 int check_cache(const llmhip_kv_cache* c) {
   ARG(c, "cache is null");
   ARG(c->dtype <= LLMHIP_E4M3, "unknown cache dtype");
@@ -190,13 +197,17 @@ int llmhip_kv_append(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
   if (T == 0) return LLMHIP_OK;
   ARG(k && v && slots, "k, v and slots are required");
   ARG(!dims || positions, "positions are required with rope");
+  const int64_t k_stride[2] = {k_token, k_head}, v_stride[2] = {v_token, v_head}, q_stride[2] = {q_token, q_head},
+                out_q_stride[2] = {out_q_token, out_q_head};
+  const uint64_t pool_extents[3] = {cache->pages, cache->page, cache->heads}, q_extents[2] = {T, q_heads};
+  ARG(rows_apart(cache->k_stride, pool_extents, 3, cache->head_dim) && rows_apart(cache->v_stride, pool_extents, 3, cache->head_dim),
+      "rows of a pool overlap");
+  ARG(!q || rows_apart(out_q_stride, q_extents, 2, cache->head_dim), "rows of out_q overlap");
   // The widest vectors that the rows' starts and the pairs' places allow: a
   // vector of 16 bytes, or of 8, or single values; of neighbouring pairs two
   // vectors are one access.
   const uint32_t elem = size_of(dtype), kv_elem = size_of(cache->dtype), dim = cache->head_dim;
   const bool neighbours = rope && rope->style == LLMHIP_ROPE_NEIGHBOURS;
-  const int64_t k_stride[2] = {k_token, k_head}, v_stride[2] = {v_token, v_head}, q_stride[2] = {q_token, q_head},
-                out_q_stride[2] = {out_q_token, out_q_head};
   uint32_t vec = (neighbours ? 8 : 16) / elem;
   for (const uint32_t least = 8 / elem; vec >= least; vec /= 2) {
     const uint32_t access = neighbours ? 2 * vec : vec, bytes = access * elem, kv_bytes = access * kv_elem;
@@ -256,6 +267,9 @@ int llmhip_kv_attend(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
   TRY(check_table(table_pages, table_ld, cache->page));
   if (B == 0) return LLMHIP_OK;
   ARG(q && out && lens, "q, out and lens are required");
+  const int64_t out_stride[2] = {out_request, out_head};
+  const uint64_t out_extents[2] = {B, q_heads};
+  ARG(rows_apart(out_stride, out_extents, 2, cache->head_dim), "rows of out overlap");
   ARG(table || table_pages == 0, "table is null");
   ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be given, aligned to 16 bytes");
   ON_DEVICE(info);

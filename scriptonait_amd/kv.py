@@ -98,6 +98,14 @@ def _rows(t, shape, dtype, name: str, device):
     return t.data_ptr(), a, b
 
 
+def _out_rows(t, shape, dtype, name: str, device):
+    """_rows of a tensor that is written."""
+    r = _rows(t, shape, dtype, name, device)
+    if (r[1] < shape[2] and shape[0] > 1) or (r[2] < shape[2] and shape[1] > 1):
+        raise ValueError(f"rows of {name} overlap")
+    return r
+
+
 def _table(t, n: int, device):
     """A block table of n requests; its address, pages and row stride."""
     if t.dtype is not torch.int32 or t.dim() != 2 or t.shape[0] != n or (t.stride(1) != 1 and t.shape[1] > 1 and n):
@@ -249,6 +257,8 @@ class KVCache:
         self._c = LlmhipKvCache(k_pool.data_ptr(), v_pool.data_ptr(), *scales, (_i64 * 3)(*k_pool.stride()[:3]),
                                 (_i64 * 3)(*v_pool.stride()[:3]), DTYPES[self.dtype], pages, page, heads, dim)
         self._ref = ctypes.addressof(self._c)
+        # Rows that lie over one another can be read, not appended to.
+        self._apart = all(s >= dim or n < 2 for p in (k_pool, v_pool) for s, n in zip(p.stride()[:3], p.shape))
         self._scale = 1.0 / math.sqrt(dim)
         self._append, self._attend = self.lib.llmhip_kv_append, self.lib.llmhip_kv_attend
         # What may come beside this cache, as the C entries name it.
@@ -265,6 +275,8 @@ class KVCache:
         code = self._codes.get(dt)
         if code is None:
             raise ValueError(f"k is {dt}, which does not go into a {self.dtype} cache")
+        if not self._apart:
+            raise ValueError("rows of a pool overlap")
         if (q is None) != (out_q is None):
             raise ValueError("q and out_q go together")
         T = slots.numel()
@@ -282,7 +294,7 @@ class KVCache:
                 raise ValueError("q must be [T, q_heads, head_dim]")
             heads = q.shape[1]
             q_shape = (T, heads, self.head_dim)
-            q_rows, out_rows = _rows(q, q_shape, dt, "q", dev), _rows(out_q, q_shape, dt, "out_q", dev)
+            q_rows, out_rows = _rows(q, q_shape, dt, "q", dev), _out_rows(out_q, q_shape, dt, "out_q", dev)
         status = self._append(
             self.sampler.ctx, self._ref, code, T, *_rows(k, shape, dt, "k", dev), *_rows(v, shape, dt, "v", dev),
             _vector(slots, T, torch.int64, "slots", dev), heads, *q_rows, *out_rows,
@@ -330,7 +342,7 @@ class KVCache:
         status = self._attend(
             self.sampler.ctx, self._ref, code, B, heads, *_rows(q, shape, dt, "q", dev), *_table(table, B, dev),
             _vector(lens, B, torch.int32, "lens", dev), window, self._scale if scale is None else scale,
-            *_rows(out, shape, dt, "out", dev), lse, _vector(workspace, size, torch.uint8, "workspace", dev), size,
+            *_out_rows(out, shape, dt, "out", dev), lse, _vector(workspace, size, torch.uint8, "workspace", dev), size,
             _current(dev) if stream is None else _on(stream, dev, (q, table, lens, out, out_lse, workspace, self.k_pool,
                                                                    self.v_pool, self.k_scale, self.v_scale)))
         if status:
