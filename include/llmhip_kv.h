@@ -110,7 +110,8 @@ typedef struct llmhip_rope {
  * too, which goes back as it is) set
  * LLMHIP_KSTATUS_BAD_INDEX: the length is clamped, the count taken as 0, the
  * pool as empty, and the token's slot is -1. Apart from out_lens and
- * out_free_state no output may overlap an input.
+ * out_free_state no output may overlap an input, and ring and table none
+ * either: refused.
  */
 int llmhip_kv_plan(llmhip_ctx* ctx, size_t pages, size_t page, int32_t* ring, const int32_t* free_state, size_t R,
                    const int32_t* lens, const int32_t* new_tokens, const int32_t* release, int32_t* table,

@@ -38,12 +38,15 @@ int launched(hipError_t e, const char* what) {
 #define SUPPORTED(cond, what) \
   if (!(cond)) return unsupported(what)
 
-// An array of n values and one of m share no memory; a null one shares none.
-bool apart(const int32_t* x, size_t n, const int32_t* y, size_t m) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
-  return !x || !y || a + n * sizeof(int32_t) <= b || b + m * sizeof(int32_t) <= a;
-}
-bool same_or_apart(const int32_t* x, const int32_t* y, size_t n) { return x == y || apart(x, n, y, n); }
+// Memory of an argument; a null one has none.
+struct Span {
+  uintptr_t at;
+  size_t bytes;
+  template <class T>
+  Span(const T* p, size_t n) : at(reinterpret_cast<uintptr_t>(p)), bytes(p ? n * sizeof(T) : 0) {}
+  bool apart(const Span& o) const { return !bytes || !o.bytes || at + bytes <= o.at || o.at + o.bytes <= at; }
+  bool same(const Span& o) const { return at == o.at && bytes == o.bytes; }
+};
 
 constexpr size_t kMaxInt = 0x7fffffff;
 constexpr size_t kMaxBatch = 65535;
@@ -149,14 +152,20 @@ int llmhip_kv_plan(llmhip_ctx* ctx, size_t pages, size_t page, int32_t* ring, co
   ARG(T == 0 || (slots && positions), "slots and positions are required");
   SUPPORTED(R <= kMaxInt - 1024 && T <= kMaxInt - 1024, "R or T too large");
   TRY(check_table(table_pages, table_ld, page));
-  ARG(same_or_apart(lens, out_lens, R), "lens and out_lens overlap");
-  ARG(same_or_apart(free_state, out_free_state, 2), "free_state and out_free_state overlap");
   ON_DEVICE(info);
-  // Workgroups read what each request asks for while others write the results.
-  for (const int32_t* in : {lens, new_tokens, release}) {
-    ARG(apart(in, R, granted, R) && apart(in, R, start, R + 1), "granted and start must not overlap what they follow from");
-    ARG(in == lens || apart(in, R, out_lens, R), "out_lens overlaps new_tokens or release");
-  }
+  // Workgroups read what each request asks for, and the tokens' pages, while
+  // others write the results.
+  const Span lens_span(lens, R), state(free_state, 2);
+  const Span table_span(table, R && table_pages ? (R - 1) * table_ld + table_pages : 0);
+  const Span inputs[] = {lens_span, {new_tokens, R}, {release, R}, state, {ring, pages}, table_span};
+  const Span outputs[] = {{out_lens, R}, {out_free_state, 2}, {granted, R}, {start, R + 1}, {slots, T}, {positions, T}};
+  for (const Span& out : outputs)
+    for (const Span& in : inputs)
+      ARG(out.apart(in) || (&out == &outputs[0] && &in == &inputs[0] && out.same(in)) ||
+              (&out == &outputs[1] && &in == &inputs[3] && out.same(in)),
+          "an output overlaps an input (only out_lens may be lens, and out_free_state free_state)");
+  for (int i = 0; i < 5; ++i)
+    ARG(inputs[i].apart(table_span) && (i == 4 || inputs[i].apart(inputs[4])), "ring or table overlaps another input");
   PlanArgs a{};
   a.ring = ring;
   a.free_state = free_state;
