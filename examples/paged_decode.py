@@ -91,12 +91,16 @@ def norm(x):
     return (y * torch.rsqrt(y.square().mean(-1, keepdim=True) + 1e-5)).to(x.dtype)
 
 
-def generate(sampler, prompts, steps, config=None, seeds=None, on_step=None, **model):
+def generate(sampler, prompts, steps, config=None, seeds=None, on_step=None, make=Decoder, **model):
     """Decodes every prompt until it and its new tokens are `steps` long, or
-    its own limit (a (prompt, limit) pair) is reached; the token lists."""
+    its own limit (a (prompt, limit) pair) is reached; the token lists. The
+    cache has room for all of them, unless `model` says how much it has."""
     prompts = [p if isinstance(p, tuple) else (p, steps) for p in prompts]
     B, dev = len(prompts), torch.device("cuda:0")
-    m = Decoder(sampler, batch=B, **model)
+    page = model.setdefault("page_size", 16)
+    model.setdefault("context", -(-steps // page) * page)
+    model.setdefault("pages", B * (model["context"] // page))
+    m = make(sampler, batch=B, **model)
     config = SamplingConfig(temperature=0.8, top_k=20, repetition_penalty=1.0) if config is None else config
     rng = torch.tensor(np.arange(B) if seeds is None else seeds, dtype=torch.int64, device=dev)
     ids = torch.zeros(B, dtype=torch.int32, device=dev)
@@ -105,8 +109,11 @@ def generate(sampler, prompts, steps, config=None, seeds=None, on_step=None, **m
         told[b, :len(p)] = torch.tensor(p, dtype=torch.int32)
     given = torch.tensor([len(p) for p, _ in prompts], device=dev)
     limit = torch.tensor([min(n, steps) for _, n in prompts], device=dev)
+    refused = torch.zeros((), dtype=torch.bool, device=dev)
     for t in range(steps):
-        slots, positions = m.plan((limit > t).int(), (limit == t).int())
+        wants = (limit > t).int()
+        slots, positions = m.plan(wants, (limit == t).int())
+        refused |= (m.granted < wants).any()
         hidden = m.forward(told[:, t].long(), slots, positions)
         if on_step is not None:
             on_step(t, hidden)
@@ -116,6 +123,8 @@ def generate(sampler, prompts, steps, config=None, seeds=None, on_step=None, **m
     torch.cuda.synchronize()
     if sampler.status().flags:
         raise RuntimeError("a kernel flagged its input")
+    if refused:  # such a token is in no cache: what followed did not see it
+        raise RuntimeError("the cache had no room for a token")
     return [told[b, :int(limit[b])].tolist() for b in range(B)], m
 
 
