@@ -5,15 +5,12 @@
 
 #include "../../include/llmhip_kv.h"
 #include "kv_index.h"
+#include "kv_split.h"
 
 namespace llmhip {
 
 constexpr uint32_t kMaxHeadDim = 256;
-// Attention: the ranges that a call's work is cut into, and the requests of a
-// call that is cut (their tiles' prefix sums live in LDS).
-constexpr uint32_t kMaxRanges = 1024;
-constexpr uint32_t kMaxSplitBatch = 2048;
-constexpr uint32_t kCutWords = 4 * kMaxRanges;  // workspace words before the partial answers
+constexpr uint32_t kCutWords = 4 * kMaxRanges;  // attention: workspace words before the partial answers
 
 struct PlanArgs {
   int32_t* ring;

@@ -337,9 +337,6 @@ __device__ __forceinline__ float lse_of(float m, float l) {
   return l == 0.0f ? -INFINITY : kLn2 * (m + __builtin_amdgcn_logf(l));
 }
 
-// Words of a partial answer: o of every query head, then m, then l.
-__host__ __device__ __forceinline__ uint32_t partial_words(uint32_t group, uint32_t dim) { return group * (dim + 2u); }
-
 template <class E, bool GROUPED, bool ONCE>
 __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(AttendArgs a) {
   constexpr uint32_t kWaves = kWavesOf<E, GROUPED>;
@@ -651,38 +648,11 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
 template <class E, bool GROUPED, bool ONCE>
 hipError_t launch_attend_group(AttendArgs a, hipStream_t s) {
   constexpr uint32_t kWaves = kWavesOf<E, GROUPED>;
-  // All waves have work: 12 heads are three teams of 4 with two waves each, not
-  // two of 6 with one (head size 96: 130 us and 135; 3 heads of 64: 17 and 19).
-  a.team = kWaves;
-  while (a.vheads % a.team) a.team /= 2u;
-  const uint32_t longest = (a.window ? min(a.table_pages * a.page, a.window + E::kTile) : a.table_pages * a.page) / E::kTile + 1u;
-  // A workgroup of 8 waves, or two of 4, on each compute unit (two and three
-  // times as many: 64 requests 104, 106, 110 us then, and 54, 80, 96 for one of
-  // 131072 tokens of a single head). More requests, or tiles, than the line
-  // takes are not cut, with a workgroup for each.
-  const uint32_t groups = a.cus * (8u / kWaves);
-  const bool cut = a.B <= kMaxSplitBatch && (uint64_t)a.B * longest <= 0x7fffffffu;
-  // Nor are requests so short that a workgroup reads one whole sooner than
-  // ranges are read and joined. The longest that the table or the window allow
-  // counts, with as many waves for each head as there are workgroups for:
-  //   up to 320 KiB a workgroup: 30 requests of up to 200 tokens of 8 heads of 128
-  //     bf16 10.1 us whole, 15.9 cut; 3 of 60 tokens 5.9 and 9.0; one of 512 tokens
-  //     of 2 heads of 64 f32 12.1 and 11.9, and one launch less.
-  //   up to 1 MiB where the workgroups fill an eighth of the card: 300 of up to 100
-  //     tokens 26.8 and 32.1, 200 of up to 1000 of one head 22.3 and 31.2. (Fewer:
-  //     one of 2000 tokens of 8 heads 29.6 and 16.1.)
-  //   up to 640 KiB there where rows are no whole cache lines: 37 of up to 1000 of
-  //     12 heads of 80 f16, 737 KiB, 39.8 and 32.5.
-  uint32_t team = a.team;
-  while (team > 1u && a.B * (a.vheads / team) < groups) team /= 2u;
-  const uint64_t takes = (uint64_t)a.B * (a.vheads / team), rounds = (takes + groups - 1u) / groups;
-  const uint64_t bytes = rounds * ((longest + kWaves / team - 1u) / (kWaves / team)) * kWaves * E::kTile * a.dim * 2u * E::kElem;
-  const uint64_t few = takes < groups / 8u ? 320u : a.dim * E::kElem % 128u ? 640u : 1024u;
-  const bool whole = !cut || bytes <= few * 1024u;
-  if (whole) a.team = team;
-  a.splits = kWaves / a.team;
+  const AttendSplit split = attend_split(kWaves, E::kTile, a.dim * 2u * E::kElem, a.cus, a.B, a.vheads, a.table_pages * a.page, a.window);
+  a.team = split.team;
+  a.splits = split.splits;
+  a.ranges = split.ranges;
   const uint32_t teams = a.vheads / a.team;
-  a.ranges = whole ? 0u : max(groups / teams, 1u);
   a.start_words = a.ranges && a.B > 64u ? 16u + (a.B + 1u + 3u) / 4u * 4u : 0u;
   const uint32_t lds = (a.start_words + (a.splits > 1u ? 2u * kWaves * a.part_words : 0u)) * 4u;
   const dim3 grid((a.ranges ? a.ranges : a.B) * teams), threads(a.team * a.splits * 64u);
