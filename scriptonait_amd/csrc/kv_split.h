@@ -33,23 +33,32 @@ inline AttendSplit attend_split(uint32_t waves, uint32_t tile, uint32_t token_by
   // takes are not cut, with a workgroup for each.
   const uint32_t groups = cus * (8u / waves);
   const bool cut = B <= kMaxSplitBatch && (uint64_t)B * longest <= 0x7fffffffu;
-  // Nor are requests so short that a workgroup reads one whole sooner than
-  // ranges are read and joined. The longest that the table or the window allow
-  // counts, with as many waves for each head as there are workgroups for:
-  //   up to 320 KiB a workgroup: 30 requests of up to 200 tokens of 8 heads of 128
-  //     bf16 10.1 us whole, 15.9 cut; 3 of 60 tokens 5.9 and 9.0; one of 512 tokens
-  //     of 2 heads of 64 f32 12.1 and 11.9, and one launch less.
-  //   up to 1 MiB where the workgroups fill an eighth of the card: 300 of up to 100
-  //     tokens 26.8 and 32.1, 200 of up to 1000 of one head 22.3 and 31.2. (Fewer:
-  //     one of 2000 tokens of 8 heads 29.6 and 16.1.)
-  //   up to 640 KiB there where rows are no whole cache lines: 37 of up to 1000 of
-  //     12 heads of 80 f16, 737 KiB, 39.8 and 32.5.
+  // Nor are requests so short that workgroups read them whole, one for each
+  // request and team, sooner than ranges are read and joined. A team is as
+  // small then as there are workgroups for. Both times, in bytes that one
+  // workgroup reads, for the longest requests that the table or the window allow:
+  //   whole: its request's tiles, of which each has the time of 12 KiB before its
+  //     bytes come, and 288 KiB; more workgroups than the card takes have turns.
+  //   cut: 1280 KiB, and a quarter of a workgroup's share of all tiles (requests
+  //     are shorter than the longest, and all waves work all of the time).
+  // Measured over 7600 calls of 1 to 400 requests, 1 to 32 heads of 16 to 256
+  // values with 1 to 32 queries each, all types, windows of 128 to 1000 tokens and
+  // none, by the quotient of the two (us: medians; measured: geometric means):
+  //   by the rule  to 0.5  -0.75     -1  -1.33     -2     -4   more
+  //   whole, us       8.1   12.9   19.4   24.3   31.5   47.3   84.8
+  //   cut, us        11.8   15.5   20.3   23.8   28.0   25.8   22.1
+  //   measured       0.70   0.84   0.95   1.06   1.18   1.64   3.87
+  // The better of the two is missed by 2.4% in the mean (all whole 14%, all cut
+  // 21%), by 2.8% over 1200 calls that the numbers were not chosen by.
   uint32_t team = cut_team;
   while (team > 1u && (uint64_t)B * (vheads / team) < groups) team /= 2u;
-  const uint64_t takes = (uint64_t)B * (vheads / team), rounds = (takes + groups - 1u) / groups;
-  const uint64_t bytes = ((uint64_t)longest + waves / team - 1u) / (waves / team) * waves * tile * token_bytes;
-  const uint64_t few = takes < groups / 8u ? 320u : token_bytes / 2u % 128u ? 640u : 1024u;
-  if (!cut || rounds == 0u || bytes <= few * 1024u / rounds) return {team, waves / team, 0u};
+  constexpr double kKiB = 1024.0;
+  const double turns = std::max((double)B * (vheads / team) / groups, 1.0);
+  const double tile_time = (double)tile * token_bytes + 12.0 * kKiB;
+  const uint32_t wave_tiles = (uint32_t)(((uint64_t)longest + waves / team - 1u) / (waves / team));
+  const double whole_time = turns * (wave_tiles * (double)waves * tile_time + 288.0 * kKiB);
+  const double cut_time = 1280.0 * kKiB + 0.25 * B * longest * vheads / groups * tile_time;
+  if (!cut || whole_time <= cut_time) return {team, waves / team, 0u};
   const uint32_t teams = vheads / cut_team;
   return {cut_team, waves / cut_team, std::min(std::max(groups / teams, 1u), kMaxRanges)};
 }

@@ -71,4 +71,4 @@ def test_scores_past_binary32_give_nan(sampler, B, n):
     c["k_pool"][id, at, 0, 0] = 3e19  # 3e38, times log2(e) past the largest number
     got = _attend(sampler, c, scale=1.0)
     assert got[0][0].isnan().all() and got[1][0].isnan().all()
-    assert got[0][1:].isfinite().all() and np.isfinite(got[1][1:]).all()
+    assert got[0][1:].isfinite().all() and got[1][1:].isfinite().all()
