@@ -666,8 +666,8 @@ hipError_t launch_attend_group(AttendArgs a, hipStream_t s) {
 
 // Values are read past the caches unless the next call may find them there (the
 // card keeps 256 MB: pools of up to 64 MiB each), or the heads beside them on
-// their cache lines do. 537 MB 99 us and 107 with plain loads, 2.2 GB of E4M3 345
-// and 378; 67 MB of one head 26.2 and 24.8, 205 MB of rows of 32 bytes 87 and 72.
+// their cache lines do. 537 MB 96 us and 102 with plain loads, 2.2 GB of E4M3 346
+// and 379; 67 MB of one head 26.4 and 24.9, 205 MB of rows of 32 bytes 89 and 75.
 template <class E>
 hipError_t launch_attend_engine(const AttendArgs& a, hipStream_t s) {
   const bool grouped = a.page % E::kGroup == 0u;
