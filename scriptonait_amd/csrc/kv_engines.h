@@ -225,16 +225,18 @@ struct Engine16 {
       for (int j = 0; j < kVec; ++j) o[p][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // Whether a sum of this lane is no finite number.
+  // Whether a value that was added is no finite number. All rows of its column
+  // are none then, whatever their weights (0 times it is NaN): one is looked at.
   __device__ __forceinline__ bool infinite() const {
-    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    float x = 0.0f, y = 0.0f;
 #pragma unroll
     for (int p = 0; p < kPanels; ++p)
 #pragma unroll
-      for (int j = 0; j < kVec; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(o[p][j][i], 0.0f, x[i]);
-    return !((x[0] + x[1]) + (x[2] + x[3]) == 0.0f);
+      for (int j = 0; j < kVec; j += 2) {
+        x = __builtin_fmaf(o[p][j][0], 0.0f, x);
+        y = __builtin_fmaf(o[p][j + 1][0], 0.0f, y);
+      }
+    return !(x + y == 0.0f);
   }
   // Of token i's values only those that are finite, or only the others.
   __device__ __forceinline__ void keep_finite(int i, bool finite) {
