@@ -229,7 +229,8 @@ class KVCache:
     head_dim], dense in their last dimension, of float32, bfloat16, float16
     or float8_e4m3fn; with the last one k_scale and v_scale ([heads] float32)
     are what a stored value is multiplied with. head_dim is a multiple of 8
-    up to 256."""
+    up to 256. Pools whose rows overlap (expanded ones) can be attended over,
+    not appended to."""
 
     def __init__(self, sampler: Sampler, k_pool, v_pool, k_scale=None, v_scale=None):
         if k_pool.dim() != 4 or k_pool.shape != v_pool.shape:
