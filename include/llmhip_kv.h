@@ -12,6 +12,9 @@
  *                      values into their slots
  *   llmhip_kv_attend   for each layer: attention over the request's pages
  *   llmhip_decode_step the sampler, on the logits of the last layer
+ * and, for a cache of 8 bits whose scales follow from what is written into it,
+ * llmhip_kv_block_append and llmhip_kv_block_attend in the place of the two
+ * in the middle, with llmhip_kv_block_read to read tokens back.
  *
  * Conventions as in llmhip_sampler.h: plain pointers and sizes, the caller
  * owns every buffer, an int status comes back, calls are stream-ordered and
@@ -34,8 +37,9 @@ extern "C" {
 /* A length, page id, slot or free-page count was outside its range. */
 #define LLMHIP_KSTATUS_BAD_INDEX 2u
 
-/* Element types. E4M3 is the 8-bit float with 4 exponent bits, no infinities. */
-enum { LLMHIP_F32 = 0, LLMHIP_BF16 = 1, LLMHIP_F16 = 2, LLMHIP_E4M3 = 3 };
+/* Element types. E4M3 is the 8-bit float with 4 exponent bits, no infinities;
+ * I8, whole numbers of 8 bits, is for llmhip_kv_blocks alone. */
+enum { LLMHIP_F32 = 0, LLMHIP_BF16 = 1, LLMHIP_F16 = 2, LLMHIP_E4M3 = 3, LLMHIP_I8 = 4 };
 
 /*
  * The cache of one layer: two pools of `pages` pages of `page` tokens, each
@@ -183,6 +187,98 @@ int llmhip_kv_attend(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
                      const void* q, int64_t q_request, int64_t q_head, const int32_t* table, size_t table_pages,
                      size_t table_ld, const int32_t* lens, size_t window, float scale, void* out, int64_t out_request,
                      int64_t out_head, float* out_lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * A cache of one layer in 8 bits, with a scale for each block of tokens and
+ * head. Pools as in llmhip_kv_cache, of type I8 or E4M3, rows aligned to 8
+ * bytes. A page is page / block blocks of `block` neighbouring tokens (block
+ * divides page and is at most 256); the scale of page p's block b and head h
+ * is at p*scale_stride[0] + b*scale_stride[1] + h*scale_stride[2] of k_scale or
+ * v_scale (device f32). A code c stands for c * scale. Scales are written by
+ * llmhip_kv_block_append and need no values before a block's first token is.
+ */
+typedef struct llmhip_kv_blocks {
+  void* k_pool;
+  void* v_pool;
+  float* k_scale;
+  float* v_scale;
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t k_scale_stride[3];
+  int64_t v_scale_stride[3];
+  uint32_t dtype;
+  uint32_t pages;
+  uint32_t page;
+  uint32_t block;
+  uint32_t heads;
+  uint32_t head_dim;
+} llmhip_kv_blocks;
+
+/*
+ * llmhip_kv_append for such a cache: k, v, q and out_q of F32, BF16 or F16;
+ * keys and queries rotated as there, in binary32.
+ *
+ * The tokens of one block that a call writes stand next to each other in the
+ * batch, in the order of their slots and without gaps, as llmhip_kv_plan gives
+ * them. (In another order, or with a slot twice, what the block then holds is
+ * undefined; nothing else is touched.) Its tokens before the first
+ * new one are kept, and for each head, with MAX 127 (I8) or 448 (E4M3),
+ *   s_new = max |x| / MAX   over the new tokens' values, after the rotation
+ *   s     = s_new where no token is kept, else max(s_old, s_new)
+ *   code  = x * (1 / s)     to the nearest, ties to even, at most MAX
+ *   kept  = c * (s_old / s) the same, where s > s_old
+ * in binary32. A value is off by half a step: s / 2 (I8), 2^-4 of itself or
+ * 2^-10 s (E4M3), and once more by as much of the new step whenever a later
+ * token of its block raises the scale. A block's scale falls when its first
+ * token is written again. An s_new below 2^-126 is 0, and codes of a scale of 0
+ * are 0. Infinite values are not looked at for s and stored as +-MAX; NaN is
+ * stored as 0 (I8) or NaN (E4M3).
+ */
+int llmhip_kv_block_append(llmhip_ctx* ctx, const llmhip_kv_blocks* cache, uint32_t dtype, size_t T, const void* k,
+                           int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                           const int64_t* slots, size_t q_heads, const void* q, int64_t q_token, int64_t q_head,
+                           void* out_q, int64_t out_q_token, int64_t out_q_head, const int32_t* positions,
+                           const llmhip_rope* rope, void* stream);
+
+/*
+ * The keys and values of T slots: each code times its scale in binary32, and
+ * that rounded to dtype (F32, BF16 or F16).
+ *
+ *   slots         device [T], in any order, also the same one twice; < 0: a
+ *                 row of zeros. One past the pool gives zeros and is flagged
+ *   out_k, out_v  device [T][heads][head_dim] with strides; either may be
+ *                 null. Rows that overlap are refused
+ */
+int llmhip_kv_block_read(llmhip_ctx* ctx, const llmhip_kv_blocks* cache, uint32_t dtype, size_t T, const int64_t* slots,
+                         void* out_k, int64_t out_k_token, int64_t out_k_head, void* out_v, int64_t out_v_token,
+                         int64_t out_v_head, void* stream);
+
+/* Bytes of workspace that llmhip_kv_block_attend takes for this cache, so many
+ * new tokens and q_heads, whatever the batch. */
+int llmhip_kv_block_attend_workspace(llmhip_ctx* ctx, const llmhip_kv_blocks* cache, size_t new_tokens, size_t q_heads,
+                                     size_t* bytes);
+
+/*
+ * llmhip_kv_attend for such a cache, and for the newest new_tokens (1 to 16)
+ * tokens of each request: token j of them is attended over the first
+ * lens[b] - new_tokens + 1 + j tokens, of those the last `window` where window
+ * is not 0. One that is attended over none gets zeros and an lse of -inf.
+ *
+ *   dtype      of q and out: BF16 or F16
+ *   q, out     device [B][new_tokens][q_heads][head_dim], a request's, a
+ *              token's and a head's stride in elements
+ *   out_lse    device nullable [B][new_tokens][q_heads] f32
+ *
+ * All else is as there. Scales of tokens that are seen have to be finite; what
+ * is behind a request's length (codes and scales) is never used. Each softmax
+ * weight times its value's scale is rounded to binary32 and meets the codes as
+ * the sum of two bfloat16: off by at most 2^-16 of itself.
+ */
+int llmhip_kv_block_attend(llmhip_ctx* ctx, const llmhip_kv_blocks* cache, uint32_t dtype, size_t B, size_t new_tokens,
+                           size_t q_heads, const void* q, int64_t q_request, int64_t q_token, int64_t q_head,
+                           const int32_t* table, size_t table_pages, size_t table_ld, const int32_t* lens,
+                           size_t window, float scale, void* out, int64_t out_request, int64_t out_token,
+                           int64_t out_head, float* out_lse, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

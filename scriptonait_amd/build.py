@@ -28,7 +28,9 @@ LIB_PATH = PKG_DIR / LIB_NAME
 SOURCES = ["sampler_kernels.hip", "vocab_full.hip", "vocab_plain.hip", "fast_nch8.hip", "fast_nch_small.hip", "fast_counts.hip", "fast_counts8.hip",
            "fast_counts_small.hip", "tied_head.hip", "bench_floor.hip", "stream_topk.hip", "stream_topk_bigk.hip", "stream_topk_refine.hip", "sampler_api.hip", "scck_reader.cpp",
            "kv_plan.hip", "kv_append.hip", "kv_attend_f32.hip", "kv_attend_bf16.hip", "kv_attend_f16.hip",
-           "kv_attend_e4m3_bf16.hip", "kv_attend_e4m3_f16.hip", "kv_api.hip"]
+           "kv_attend_e4m3_bf16.hip", "kv_attend_e4m3_f16.hip", "kv_api.hip",
+           "kv_block_append.hip", "kv_block_read.hip", "kv_block_attend_i8_bf16.hip", "kv_block_attend_i8_f16.hip",
+           "kv_block_attend_e4m3_bf16.hip", "kv_block_attend_e4m3_f16.hip", "kv_block_api.hip"]
 ARCH = "gfx950"
 
 

@@ -1,73 +1,14 @@
 // C entry points of the paged key-value cache (declared in
-// include/llmhip_kv.h): what the host can check, and the launches. Arguments
-// are checked before the context, so a wrong call says what is wrong with it
-// also where there is no device.
+// include/llmhip_kv.h): what the host can check, and the launches.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
-#include <stdio.h>
 #include <string.h>
 
-#include <algorithm>
-
-#include "ctx_info.h"
-#include "device_scope.h"
-#include "kv_args.h"
+#include "kv_check.h"
 
 using namespace llmhip;
 
 namespace {
-
-int arg_fail(const char* what) {
-  set_last_error(what);
-  return LLMHIP_ERR_INVALID_ARGUMENT;
-}
-int unsupported(const char* what) {
-  set_last_error(what);
-  return LLMHIP_ERR_UNSUPPORTED;
-}
-int launched(hipError_t e, const char* what) {
-  if (e == hipSuccess) return LLMHIP_OK;
-  char buf[256];
-  snprintf(buf, sizeof buf, "%s: %s (%d)", what, hipGetErrorString(e), (int)e);
-  set_last_error(buf);
-  return e == hipErrorOutOfMemory ? LLMHIP_ERR_OUT_OF_MEMORY : LLMHIP_ERR_HIP;
-}
-
-#define ARG(cond, what) \
-  if (!(cond)) return arg_fail(what)
-#define SUPPORTED(cond, what) \
-  if (!(cond)) return unsupported(what)
-
-// Memory of an argument; a null one has none.
-struct Span {
-  uintptr_t at;
-  size_t bytes;
-  template <class T>
-  Span(const T* p, size_t n) : at(reinterpret_cast<uintptr_t>(p)), bytes(p ? n * sizeof(T) : 0) {}
-  bool apart(const Span& o) const { return !bytes || !o.bytes || at + bytes <= o.at || o.at + o.bytes <= at; }
-  bool same(const Span& o) const { return at == o.at && bytes == o.bytes; }
-};
-
-constexpr size_t kMaxInt = 0x7fffffff;
-constexpr size_t kMaxBatch = 65535;
-constexpr size_t kMaxHeads = 65535;
-
-uint32_t size_of(uint32_t dtype) { return dtype == LLMHIP_F32 ? 4u : dtype == LLMHIP_E4M3 ? 1u : 2u; }
-
-// Whether every row of an operand starts on `bytes`.
-bool rows_on(const void* p, const int64_t* strides, int n, uint32_t elem, uint32_t bytes) {
-  if (reinterpret_cast<uintptr_t>(p) % bytes) return false;
-  for (int i = 0; i < n; ++i)
-    if ((uint64_t)strides[i] * elem % bytes) return false;
-  return true;
-}
-
-// Whether neighbours in each direction have `dim` values to themselves.
-bool rows_apart(const int64_t* strides, const uint64_t* extents, int n, uint32_t dim) {
-  for (int i = 0; i < n; ++i)
-    if (extents[i] > 1 && strides[i] < (int64_t)dim && strides[i] > -(int64_t)dim) return false;
-  return true;
-}
 
 int check_cache(const llmhip_kv_cache* c) {
   ARG(c, "cache is null");
@@ -91,40 +32,6 @@ int check_dtype(const llmhip_kv_cache* c, uint32_t dtype) {
   ARG(dtype == c->dtype || c->dtype == LLMHIP_E4M3, "dtype is neither the cache's nor beside an E4M3 cache");
   return LLMHIP_OK;
 }
-
-int check_table(size_t table_pages, size_t table_ld, size_t page) {
-  ARG(table_ld >= table_pages, "table_ld < table_pages");
-  SUPPORTED(table_pages <= kMaxInt && (table_pages + 1) * page <= kMaxInt - 256, "table_pages * page must be below 2^31");
-  return LLMHIP_OK;
-}
-
-#define TRY(expr)                       \
-  do {                                  \
-    const int st_ = (expr);             \
-    if (st_ != LLMHIP_OK) return st_;   \
-  } while (0)
-
-#define ON_DEVICE(info)                                                    \
-  ARG(ctx, "ctx is null");                                                 \
-  const CtxInfo info = ctx_info(ctx);                                      \
-  Device scope(info.device);                                               \
-  if (!scope.ok) return launched(hipErrorInvalidDevice, "hipSetDevice")
-
-// Sizes of llmhip_kv_attend's work and workspace.
-struct AttendPlan {
-  uint32_t group, blocks, vheads, part_words;
-  size_t parts;  // partial answers: two for each range and block of query heads
-  AttendPlan(const llmhip_kv_cache* c, size_t q_heads, uint32_t cus) {
-    group = (uint32_t)q_heads / c->heads;
-    blocks = (group + 15u) / 16u;
-    vheads = blocks * c->heads;
-    part_words = (std::min(group, 16u) * (c->head_dim + 2u) + 3u) / 4u * 4u;
-    // Workgroups of up to 8 blocks fill the card, or two of up to 4: a range
-    // for each 8 of the blocks at most, and one range at least.
-    parts = 2 * std::max<size_t>(vheads, (size_t)8 * cus);
-  }
-  size_t bytes() const { return (kCutWords + parts * part_words) * 4; }
-};
 
 void set_pools(const llmhip_kv_cache* c, const void** pool, const float** scale, int64_t (*stride)[3]) {
   pool[0] = c->k_pool;
@@ -260,7 +167,7 @@ int llmhip_kv_attend_workspace(llmhip_ctx* ctx, const llmhip_kv_cache* cache, si
   ARG(q_heads >= 1 && q_heads % cache->heads == 0, "q_heads must be a multiple of the cache's heads");
   SUPPORTED(q_heads <= kMaxHeads, "q_heads too large");
   ARG(ctx, "ctx is null");
-  *bytes = AttendPlan(cache, q_heads, ctx_info(ctx).cus).bytes();
+  *bytes = AttendPlan(cache->heads, cache->head_dim, q_heads, ctx_info(ctx).cus).bytes();
   return LLMHIP_OK;
 }
 
@@ -282,7 +189,7 @@ int llmhip_kv_attend(llmhip_ctx* ctx, const llmhip_kv_cache* cache, uint32_t dty
   ARG(table || table_pages == 0, "table is null");
   ARG(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "workspace must be given, aligned to 16 bytes");
   ON_DEVICE(info);
-  const AttendPlan plan(cache, q_heads, info.cus);
+  const AttendPlan plan(cache->heads, cache->head_dim, q_heads, info.cus);
   ARG(workspace_bytes >= plan.bytes(), "workspace is smaller than llmhip_kv_attend_workspace says");
   AttendArgs a{};
   a.q = q;

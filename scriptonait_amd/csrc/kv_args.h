@@ -49,6 +49,35 @@ struct AppendArgs {
   double freqs[kMaxHeadDim / 2];
 };
 
+// For each block of tokens and head: where its scale is, and which block a
+// token of a page is in.
+struct BlockScales {
+  float* scale[2];
+  int64_t stride[2][3];  // page, block, head
+  FastDiv by_block;
+};
+
+struct BlockAppendArgs : AppendArgs {
+  BlockScales block_scales;
+  uint32_t kv_groups, kv_parts;  // workgroups of the keys and values: groups of tokens, and workgroups for each
+  uint32_t kv_tokens;            // tokens of such a group
+  uint32_t kv_waves;             // heads of such a workgroup
+  uint32_t turn_tokens;          // tokens whose cosines and sines LDS holds
+};
+
+struct BlockReadArgs {
+  void* out[2];  // nullable
+  const void* pool[2];
+  int64_t out_stride[2][2];
+  int64_t pool_stride[2][3];
+  BlockScales block_scales;
+  const int64_t* slots;
+  uint32_t T, heads, dim, pages, page;
+  FastDiv by_token, by_row;  // units of a token, units of a head row
+  uint32_t tokens_per_group;
+  uint32_t* status;
+};
+
 struct AttendArgs {
   const void* q;
   void* out;
@@ -74,13 +103,30 @@ struct AttendArgs {
   uint32_t* status;
 };
 
+// A cache head's queries are those of all new tokens: `group` and `q_heads`
+// count them, a query is number token * per_token + head of its cache head.
+struct BlockAttendArgs : AttendArgs {
+  BlockScales block_scales;
+  int64_t q_token, out_token;  // strides
+  uint32_t tokens, per_token;
+  uint32_t seen_window;  // of one token; `window` is that of all of them
+  FastDiv by_per_token;
+};
+
 hipError_t launch_kv_plan(const PlanArgs& a, hipStream_t s);
 hipError_t launch_kv_append(const AppendArgs& a, uint32_t dtype, uint32_t kv_dtype, bool neighbours, uint32_t vec,
                             hipStream_t s);
+hipError_t launch_kv_block_append(const BlockAppendArgs& a, uint32_t dtype, uint32_t kv_dtype, bool neighbours, uint32_t vec,
+                                  hipStream_t s);
+hipError_t launch_kv_block_read(const BlockReadArgs& a, uint32_t dtype, uint32_t kv_dtype, hipStream_t s);
 hipError_t launch_attend_f32(const AttendArgs& a, hipStream_t s);
 hipError_t launch_attend_bf16(const AttendArgs& a, hipStream_t s);
 hipError_t launch_attend_f16(const AttendArgs& a, hipStream_t s);
 hipError_t launch_attend_e4m3_bf16(const AttendArgs& a, hipStream_t s);
 hipError_t launch_attend_e4m3_f16(const AttendArgs& a, hipStream_t s);
+hipError_t launch_block_attend_i8_bf16(const BlockAttendArgs& a, hipStream_t s);
+hipError_t launch_block_attend_i8_f16(const BlockAttendArgs& a, hipStream_t s);
+hipError_t launch_block_attend_e4m3_bf16(const BlockAttendArgs& a, hipStream_t s);
+hipError_t launch_block_attend_e4m3_f16(const BlockAttendArgs& a, hipStream_t s);
 
 }  // namespace llmhip

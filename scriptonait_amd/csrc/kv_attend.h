@@ -24,6 +24,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "kv_args.h"
 #include "kv_engines.h"
 #include "wave_ops.h"
@@ -32,7 +34,7 @@ namespace llmhip {
 
 // Waves of a workgroup: 8, two on each SIMD, where the registers allow it.
 template <class E, bool GROUPED>
-constexpr uint32_t kWavesOf = E::kDim > 128 || (!GROUPED && E::kDim > 64) ? 4 : 8;
+constexpr uint32_t kWavesOf = E::kDim > 128 || (!GROUPED && E::kDim > 64) || E::kLarge ? 4 : 8;
 constexpr float kLazyBits = 8.0f;
 constexpr float kLn2 = 0.693147180559945309f, kLog2e = 1.44269504088896341f;
 constexpr uint32_t kNoId = 0xffffffffu;
@@ -119,13 +121,51 @@ struct Cut {
   uint32_t request, first, last, unused;
 };
 
+// The scales of a lane's group of tokens, of a cache that has one for each
+// block of tokens and head: N of keys and N of values, and where the cache
+// head's begin.
+template <int N>
+struct GroupScales {
+  float k[N], v[N], now[N];  // (now: of the tile at hand, times that of all scores)
+  const float* base[2];
+};
+struct NoScales {};
+template <class E>
+constexpr int scales_of() {
+  if constexpr (E::kBlocks) return E::kEach ? E::kGroup : 1;
+  else return 0;
+}
+
+// Query `qhead` of all of a request's (their number counts a cache head's
+// queries, `head`'s begin at first): its row, and its place in the request's
+// log-sum-exps. Several new tokens' queries of a cache head are its tokens' one
+// after the other.
+__device__ __forceinline__ int64_t query_row(const AttendArgs&, const int64_t* stride, int64_t, uint32_t, uint32_t qhead) {
+  return (int64_t)qhead * stride[1];
+}
+__device__ __forceinline__ uint32_t query_lse(const AttendArgs&, uint32_t, uint32_t qhead) { return qhead; }
+__device__ __forceinline__ int64_t query_row(const BlockAttendArgs& a, const int64_t* stride, int64_t token_stride, uint32_t head,
+                                             uint32_t qhead) {
+  const uint32_t i = qhead - head * a.group, token = a.by_per_token.div(i);
+  return (int64_t)token * token_stride + (int64_t)(head * a.per_token + (i - token * a.per_token)) * stride[1];
+}
+__device__ __forceinline__ uint32_t query_lse(const BlockAttendArgs& a, uint32_t head, uint32_t qhead) {
+  const uint32_t i = qhead - head * a.group, token = a.by_per_token.div(i);
+  return (token * a.heads + head) * a.per_token + (i - token * a.per_token);
+}
+__device__ __forceinline__ int64_t q_token(const AttendArgs&) { return 0; }
+__device__ __forceinline__ int64_t q_token(const BlockAttendArgs& a) { return a.q_token; }
+__device__ __forceinline__ int64_t out_token(const AttendArgs&) { return 0; }
+__device__ __forceinline__ int64_t out_token(const BlockAttendArgs& a) { return a.out_token; }
+
 // GROUPED: pages are whole groups of tokens. ONCE: values are not found in a
 // cache again.
 template <class E, bool GROUPED, bool ONCE>
 struct Run {
   static constexpr int kIds = GROUPED ? 1 : E::kGroup;       // page ids of the lane's V tokens
   static constexpr int kKIds = GROUPED ? 1 : E::kProducts;   // and of its K tokens
-  const AttendArgs& a;
+  static constexpr int kScales = scales_of<E>();
+  const typename E::Args& a;
   const int32_t* row;   // the request's table
   const char* base[2];  // the pools at the cache head
   uint32_t g, c, lo, hi;  // the lane, and the tokens that are seen
@@ -139,7 +179,10 @@ struct Run {
     uint32_t k[kKIds], v[kIds];
   };
 
-  __device__ __forceinline__ Run(const AttendArgs& args) : a(args) {}
+  std::conditional_t<E::kBlocks, GroupScales<kScales ? kScales : 1>, NoScales> scales;
+  int lane_lo, lane_hi;  // kBlocks: the tokens that the lane's query sees
+
+  __device__ __forceinline__ Run(const typename E::Args& args) : a(args) {}
 
   // First of the lane's tokens in a tile: V's group, and K's in product p.
   __device__ __forceinline__ uint32_t v_token(uint32_t t0) const { return t0 + E::kGroup * g; }
@@ -186,10 +229,24 @@ struct Run {
       for (int i = 0; i < E::kGroup; ++i) e.template load_v<ONCE>(i, token_row(1, x.v[i], a.by_page.mod(t + i)), c, a.dim);
     }
   }
-  // Which of the lane's tokens are seen, as bits; kAll in every lane of most tiles.
-  static constexpr uint32_t kAll = (1u << E::kGroup) - 1u;
+  // A scale of each of the lane's tokens, or one for all of them.
+  __device__ __forceinline__ void load_scales(float* x, int pool, uint32_t t0, const Ids& ids) const {
+    if constexpr (E::kBlocks) {
+      const uint32_t in_page = a.by_page.mod(v_token(t0));
+#pragma unroll
+      for (int i = 0; i < kScales; ++i) {
+        const uint32_t id = ids.v[GROUPED ? 0 : i], t = GROUPED ? in_page + i : a.by_page.mod(v_token(t0) + i);
+        x[i] = scales.base[pool][(int64_t)(id < a.pages ? id : 0u) * a.block_scales.stride[pool][0] +
+                                 (int64_t)a.block_scales.by_block.div(t) * a.block_scales.stride[pool][1]];
+      }
+    }
+  }
+  // Which of the lane's tokens are seen, as bits; kAll in every lane of most
+  // tiles. kBlocks: by the lane's query, and above those bits by any query.
+  static constexpr uint32_t kAll = (1u << (E::kBlocks ? 2 : 1) * E::kGroup) - 1u;
   __device__ __forceinline__ uint32_t seen_of(uint32_t t0, const Ids& x) {
     bool outside = t0 < lo || t0 + E::kTile > hi;
+    if constexpr (E::kBlocks) outside = (int)t0 < lane_lo || (int)(t0 + E::kTile) > lane_hi || outside;
 #pragma unroll
     for (int i = 0; i < kIds; ++i) outside = outside || x.v[i] >= a.pages;
     if (!__any(outside)) return kAll;
@@ -199,7 +256,12 @@ struct Run {
       const uint32_t t = v_token(t0) + i, id = x.v[GROUPED ? 0 : i];
       const bool in = t >= lo && t < hi;
       bad = bad || (in && id >= a.pages);
-      seen |= in && id < a.pages ? 1u << i : 0u;
+      if constexpr (E::kBlocks) {
+        seen |= in && id < a.pages ? 1u << (E::kGroup + i) : 0u;
+        seen |= in && id < a.pages && (int)t >= lane_lo && (int)t < lane_hi ? 1u << i : 0u;
+      } else {
+        seen |= in && id < a.pages ? 1u << i : 0u;
+      }
     }
     return seen;
   }
@@ -223,7 +285,9 @@ struct Run {
     const Ids now = fetch_ids(t0);
     Ids next = fetch_ids(min(t0 + E::kTile, t_last));
     load_keys(t0, now);
+    if constexpr (E::kBlocks) load_scales(scales.k, 0, t0, now);
     load_values(t0, now);
+    if constexpr (E::kBlocks) load_scales(scales.v, 1, t0, now);
     uint32_t seen = seen_of(t0, now);
     bool more;
     do {
@@ -233,8 +297,14 @@ struct Run {
       const uint32_t t1 = min(t0 + E::kTile, t_last);
       const Ids after = fetch_ids(min(t0 + 2u * E::kTile, t_last));
       load_keys(t1, next);
+      if constexpr (E::kBlocks) {
+#pragma unroll
+        for (int i = 0; i < kScales; ++i) scales.now[i] = scales.k[i] * scale;
+        load_scales(scales.k, 0, t1, next);
+      }
       add(s, seen);
       load_values(t1, next);
+      if constexpr (E::kBlocks) load_scales(scales.v, 1, t1, next);
       seen = seen_of(t1, next);
       next = after;
       t0 = t1;
@@ -255,13 +325,20 @@ struct Run {
     return false;
   }
 
+  // What token i's score is multiplied with.
+  static constexpr int kStep = kScales > 1 ? 1 : 0;
+  __device__ __forceinline__ float scale_of(int i) const {
+    if constexpr (E::kBlocks) return scales.now[i * kStep];
+    else return scale;
+  }
+
   // A tile's scores and values into ref, sum and o.
   __device__ __forceinline__ void add(float* s, uint32_t seen) {
     const bool edge = __any(seen != kAll) || (E::kInfinities && values != kAllValues);
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < E::kGroup; ++i) {
-      const float x = s[i] * scale;
+      const float x = s[i] * scale_of(i);
       top = fmaxf(top, !edge || (seen >> i & 1u) ? x : -INFINITY);
     }
     if (__any(top > limit)) raise(top);
@@ -273,13 +350,13 @@ struct Run {
     if (__builtin_expect(far, 0)) {
 #pragma unroll
       for (int i = 0; i < E::kGroup; ++i) {
-        s[i] = s[i] * scale - ref;
+        s[i] = s[i] * scale_of(i) - ref;
         // (The limit is rounded too: by a last bit of 16 to past the largest F16.)
         if (E::kLift > 0.0f) s[i] = s[i] > E::kLift + kLazyBits ? E::kLift + kLazyBits : s[i];
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < E::kGroup; ++i) s[i] = __builtin_fmaf(s[i], scale, -ref);
+      for (int i = 0; i < E::kGroup; ++i) s[i] = __builtin_fmaf(s[i], scale_of(i), -ref);
     }
 #pragma unroll
     for (int i = 0; i < E::kGroup; ++i) s[i] = __builtin_amdgcn_exp2f(s[i]);
@@ -288,7 +365,17 @@ struct Run {
       for (int i = 0; i < E::kGroup; ++i) {
         const bool keep = seen >> i & 1u;
         s[i] = keep ? s[i] : 0.0f;
-        e.keep_v(i, keep);
+        if constexpr (E::kBlocks) {
+          // (Whole numbers are finite whatever a place holds.)
+          const bool any = seen >> (E::kGroup + i) & 1u;
+          if constexpr (!std::is_same_v<typename E::KV, I8>) e.keep_v(i, any);
+          if (E::kEach) scales.v[i * kStep] = any ? scales.v[i * kStep] : 0.0f;
+        } else {
+          e.keep_v(i, keep);
+        }
+      }
+      if constexpr (E::kBlocks) {
+        if (!E::kEach) scales.v[0] = seen >> E::kGroup ? scales.v[0] : 0.0f;
       }
       if constexpr (E::kInfinities) {
         if (__builtin_expect(values != kAllValues, 0)) {
@@ -303,6 +390,10 @@ struct Run {
     }
 #pragma unroll
     for (int i = 0; i < E::kGroup; ++i) sum += s[i];
+    if constexpr (E::kBlocks) {
+#pragma unroll
+      for (int i = 0; i < E::kGroup; ++i) s[i] *= scales.v[i * kStep];
+    }
     e.accumulate(s);
   }
 
@@ -338,7 +429,7 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 }
 
 template <class E, bool GROUPED, bool ONCE>
-__global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(AttendArgs a) {
+__device__ __forceinline__ void attend(typename E::Args a) {
   constexpr uint32_t kWaves = kWavesOf<E, GROUPED>;
   extern __shared__ uint32_t s_mem[];
   __shared__ int32_t s_slot[2 * kWaves];  // the request of each partial answer, or -1
@@ -378,10 +469,22 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     run.base[i] = static_cast<const char*>(a.pool[i]) + (int64_t)head * a.pool_stride[i][2] * E::kElem;
-  const bool e4m3 = E::KV::kId == LLMHIP_E4M3;
+  const bool e4m3 = E::KV::kId == LLMHIP_E4M3 && !E::kBlocks;  // (blocks: the scales are the tokens')
   run.scale = a.score_scale * kLog2e * (e4m3 ? a.scale[0][head] : 1.0f);
   const float vscale = e4m3 ? a.scale[1][head] : 1.0f;
-  const uint32_t qhead = head * a.group + q0;  // of the output
+  if constexpr (E::kBlocks) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) run.scales.base[i] = a.block_scales.scale[i] + (int64_t)head * a.block_scales.stride[i][2];
+  }
+  const uint32_t qhead = head * a.group + q0;  // the first of the output
+  const auto out_of = [&](uint32_t r, uint32_t qi) {
+    return static_cast<typename E::Q::Raw*>(a.out) + (int64_t)r * a.out_stride[0] +
+           query_row(a, a.out_stride, out_token(a), head, qhead + qi);
+  };
+  const auto lse_at = [&](uint32_t r, uint32_t qi) {
+    if constexpr (E::kBlocks) return a.lse + (uint64_t)r * a.q_heads + query_lse(a, head, qhead + qi);
+    else return a.lse + (uint64_t)r * a.q_heads + qhead + qi;
+  };
 
   const auto partial_of = [&](bool before) {
     return a.workspace + a.part_offset + (((uint64_t)range * a.vheads + vhead) * 2u + (before ? 0u : 1u)) * a.part_words;
@@ -425,8 +528,12 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
     run.row = a.table + (uint64_t)b * a.table_ld;
     run.lo = window_start(len, a.window);
     run.hi = len;
+    if constexpr (E::kBlocks) {
+      run.lane_hi = (int)len + 1 - (int)a.tokens + (int)a.by_per_token.div(q0 + min(run.c, group - 1u));
+      run.lane_lo = a.seen_window ? max(run.lane_hi - (int)a.seen_window, 0) : 0;
+    }
     const typename E::Q::Raw* q = static_cast<const typename E::Q::Raw*>(a.q) + (int64_t)b * a.q_stride[0] +
-                                  (int64_t)(qhead + (run.c < group ? run.c : 0u)) * a.q_stride[1];
+                                  query_row(a, a.q_stride, q_token(a), head, qhead + (run.c < group ? run.c : 0u));
     run.e.load_q(q, run.g, a.dim, run.c < group);
     run.tiles(zero_tile + (tile - from), zero_tile + (last - from));
     if (run.again()) continue;
@@ -438,8 +545,7 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
         const uint32_t qi = 4u * run.g + i;
         const float scale = __shfl(inv, qi, 64);
         if (qi >= group) continue;
-        typename E::Q::Raw* out = static_cast<typename E::Q::Raw*>(a.out) + (int64_t)b * a.out_stride[0] +
-                                  (int64_t)(qhead + qi) * a.out_stride[1];
+        typename E::Q::Raw* out = out_of(b, qi);
 #pragma unroll
         for (uint32_t p = 0; p < E::kPanels; ++p) {
           const uint32_t d = (p * 16u + run.c) * E::kVec;
@@ -450,7 +556,7 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
           __builtin_memcpy(out + d, x.v, sizeof x.v);
         }
       }
-      if (a.lse && lane < group) a.lse[(uint64_t)b * a.q_heads + qhead + lane] = lse_of(m, l);
+      if (a.lse && lane < group) *lse_at(b, lane) = lse_of(m, l);
     } else if (a.splits > 1u) {
       put_partial(s_part + slot * a.part_words, m, l);
       if (lane == 0u) s_slot[slot] = (int32_t)b;
@@ -467,9 +573,8 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
   const auto empty = [&](uint32_t r) {
     for (uint32_t x = lane; x < group * a.dim; x += 64u) {
       const uint32_t qi = a.by_dim.div(x), d = x - qi * a.dim;
-      static_cast<typename E::Q::Raw*>(a.out)[(int64_t)r * a.out_stride[0] + (int64_t)(qhead + qi) * a.out_stride[1] + d] =
-          E::Q::store(0.0f);
-      if (a.lse && d == 0u) a.lse[(uint64_t)r * a.q_heads + qhead + qi] = -INFINITY;
+      out_of(r, qi)[d] = E::Q::store(0.0f);
+      if (a.lse && d == 0u) *lse_at(r, qi) = -INFINITY;
     }
   };
   if (a.ranges) {
@@ -541,13 +646,20 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
         }
       } else {
         const float inv = l == 0.0f ? 0.0f : vscale / l;
-        typename E::Q::Raw* out = static_cast<typename E::Q::Raw*>(a.out) + (int64_t)r * a.out_stride[0] +
-                                  (int64_t)(qhead + qi) * a.out_stride[1];
-        out[d] = E::Q::store(o * inv);
-        if (a.lse && d == 0u) a.lse[(uint64_t)r * a.q_heads + qhead + qi] = lse_of(m, l);
+        out_of(r, qi)[d] = E::Q::store(o * inv);
+        if (a.lse && d == 0u) *lse_at(r, qi) = lse_of(m, l);
       }
     }
   }
+}
+
+template <class E, bool GROUPED, bool ONCE>
+__global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(AttendArgs a) {
+  attend<E, GROUPED, ONCE>(a);
+}
+template <class E, bool GROUPED, bool ONCE>
+__global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void block_attend_kernel(BlockAttendArgs a) {
+  attend<E, GROUPED, ONCE>(a);
 }
 
 // The answers of requests that several ranges share. Row y of the grid is the
@@ -557,8 +669,8 @@ __global__ __launch_bounds__((kWavesOf<E, GROUPED> * 64)) void attend_kernel(Att
 // neighbouring quads, and where that leaves threads over, they take other
 // parts of the same quads. The order of joining follows from the number of
 // parts alone.
-template <class Q, class KV>
-__global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
+template <class Q, class KV, class Args>
+__global__ __launch_bounds__(256) void join_kernel(Args a) {
   constexpr uint32_t kBatch = 8;
   __shared__ float s_m[256], s_l[256];
   __shared__ f32x4 s_o[256];
@@ -635,18 +747,19 @@ __global__ __launch_bounds__(256) void join_kernel(AttendArgs a) {
     m = whole;
   }
   if (quad >= quads) return;
-  const float vscale = KV::kId == LLMHIP_E4M3 ? a.scale[1][head] : 1.0f, inv = l == 0.0f ? 0.0f : vscale / l;
+  const bool scaled = KV::kId == LLMHIP_E4M3 && std::is_same_v<Args, AttendArgs>;
+  const float vscale = scaled ? a.scale[1][head] : 1.0f, inv = l == 0.0f ? 0.0f : vscale / l;
   Pack<Q, 4> y;
 #pragma unroll
   for (int j = 0; j < 4; ++j) y.v[j] = Q::store(o[j] * inv);
-  typename Q::Raw* out =
-      static_cast<typename Q::Raw*>(a.out) + (int64_t)cut.request * a.out_stride[0] + (int64_t)qh * a.out_stride[1] + d;
+  typename Q::Raw* out = static_cast<typename Q::Raw*>(a.out) + (int64_t)cut.request * a.out_stride[0] +
+                         query_row(a, a.out_stride, out_token(a), head, qh) + d;
   __builtin_memcpy(out, y.v, sizeof y.v);
-  if (a.lse && d == 0u) a.lse[(uint64_t)cut.request * a.q_heads + qh] = lse_of(m, l);
+  if (a.lse && d == 0u) a.lse[(uint64_t)cut.request * a.q_heads + query_lse(a, head, qh)] = lse_of(m, l);
 }
 
 template <class E, bool GROUPED, bool ONCE>
-hipError_t launch_attend_group(AttendArgs a, hipStream_t s) {
+hipError_t launch_attend_group(typename E::Args a, hipStream_t s) {
   constexpr uint32_t kWaves = kWavesOf<E, GROUPED>;
   const AttendSplit split = attend_split(kWaves, E::kTile, a.dim * 2u * E::kElem, a.cus, a.B, a.vheads, a.table_pages * a.page, a.window);
   a.team = split.team;
@@ -656,11 +769,12 @@ hipError_t launch_attend_group(AttendArgs a, hipStream_t s) {
   a.start_words = a.ranges && a.B > 64u ? 16u + (a.B + 1u + 3u) / 4u * 4u : 0u;
   const uint32_t lds = (a.start_words + (a.splits > 1u ? 2u * kWaves * a.part_words : 0u)) * 4u;
   const dim3 grid((a.ranges ? a.ranges : a.B) * teams), threads(a.team * a.splits * 64u);
-  hipLaunchKernelGGL((attend_kernel<E, GROUPED, ONCE>), grid, threads, lds, s, a);
+  if constexpr (E::kBlocks) hipLaunchKernelGGL((block_attend_kernel<E, GROUPED, ONCE>), grid, threads, lds, s, a);
+  else hipLaunchKernelGGL((attend_kernel<E, GROUPED, ONCE>), grid, threads, lds, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.ranges < 2u) return e;
   const uint32_t quads = a.q_heads * (a.dim / 4u);
-  hipLaunchKernelGGL((join_kernel<typename E::Q, typename E::KV>), dim3((quads + 255u) / 256u, a.ranges - 1u), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((join_kernel<typename E::Q, typename E::KV, typename E::Args>), dim3((quads + 255u) / 256u, a.ranges - 1u), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
@@ -669,7 +783,7 @@ hipError_t launch_attend_group(AttendArgs a, hipStream_t s) {
 // their cache lines do. 537 MB 96 us and 102 with plain loads, 2.2 GB of E4M3 346
 // and 379; 67 MB of one head 26.4 and 24.9, 205 MB of rows of 32 bytes 89 and 75.
 template <class E>
-hipError_t launch_attend_engine(const AttendArgs& a, hipStream_t s) {
+hipError_t launch_attend_engine(const typename E::Args& a, hipStream_t s) {
   const bool grouped = a.page % E::kGroup == 0u;
   if constexpr (E::kDim == 32) {
     return grouped ? launch_attend_group<E, true, false>(a, s) : launch_attend_group<E, false, false>(a, s);
@@ -682,8 +796,8 @@ hipError_t launch_attend_engine(const AttendArgs& a, hipStream_t s) {
 
 // ENGINE<DIM, FULL>: the smallest DIM that holds head_dim. (Its name is part of
 // this function's symbol: each source needs one of its own.)
-template <template <int, bool> class ENGINE>
-hipError_t launch_attend_dims(const AttendArgs& a, hipStream_t s) {
+template <template <int, bool> class ENGINE, class Args = AttendArgs>
+hipError_t launch_attend_dims(const Args& a, hipStream_t s) {
   if (a.dim == 64u) return launch_attend_engine<ENGINE<64, true>>(a, s);
   if (a.dim == 128u) return launch_attend_engine<ENGINE<128, true>>(a, s);
   if (a.dim <= 32u) return launch_attend_engine<ENGINE<32, false>>(a, s);

@@ -1,0 +1,17 @@
+// Attention of bf16 queries over whole numbers of 8 bits with a scale for each block.
+#include "kv_block_attend.h"
+
+namespace llmhip {
+
+template <int DIM, bool FULL>
+using BlockI8BF16Wide = BlockEngine<BF16, I8, DIM, FULL, DIM == 32 ? 8 : 16, false>;
+template <int DIM, bool FULL>
+using BlockI8BF16WideEach = BlockEngine<BF16, I8, DIM, FULL, DIM == 32 ? 8 : 16, true>;
+template <int DIM, bool EACH>
+using BlockI8BF16Narrow = BlockEngine<BF16, I8, DIM, false, 8, EACH>;
+
+hipError_t launch_block_attend_i8_bf16(const BlockAttendArgs& a, hipStream_t s) {
+  return launch_block_attend<BlockI8BF16Wide, BlockI8BF16WideEach, BlockI8BF16Narrow>(a, s);
+}
+
+}  // namespace llmhip

@@ -1,0 +1,78 @@
+// Tokens' keys and values out of a cache of codes (llmhip_kv_block_read).
+//
+// A thread takes 8 codes of one head row, key or value: one load of 8 bytes,
+// one scale that the row's other threads read too, 16 or 32 bytes out. What
+// bounds it is the traffic.
+#include "kv_args.h"
+#include "kv_types.h"
+
+namespace llmhip {
+namespace {
+
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kMaxTokens = 32;
+
+template <class X, class KV>
+__global__ __launch_bounds__(kThreads) void block_read_kernel(BlockReadArgs a) {
+  __shared__ uint32_t s_page[kMaxTokens], s_token[kMaxTokens];
+  const uint32_t tid = threadIdx.x, t0 = blockIdx.x * a.tokens_per_group, n = min(a.tokens_per_group, a.T - t0);
+  if (tid < n) {
+    uint32_t p = 0, t = 0;
+    bool bad = false;
+    const bool live = split_slot(a.slots[t0 + tid], a.pages, a.page, p, t, bad);
+    if (bad) atomicOr(a.status, LLMHIP_KSTATUS_BAD_INDEX);
+    s_page[tid] = live ? p : 0xffffffffu;
+    s_token[tid] = t;
+  }
+  __syncthreads();
+  for (uint32_t u = tid; u < n * a.by_token.d; u += kThreads) {
+    const uint32_t t = a.by_token.div(u), in_token = u - t * a.by_token.d, page = s_page[t], token = s_token[t];
+    uint32_t head = a.by_row.div(in_token);
+    const uint32_t d = (in_token - head * a.by_row.d) * 8u;
+    const uint32_t kind = head >= a.heads || !a.out[0] ? 1u : 0u;
+    head -= head >= a.heads ? a.heads : 0u;
+    Pack<KV, 8> in{};
+    float scale = 0.0f;
+    if (page != 0xffffffffu) {
+      in = *reinterpret_cast<const Pack<KV, 8>*>(static_cast<const typename KV::Raw*>(a.pool[kind]) +
+                                                 (int64_t)page * a.pool_stride[kind][0] +
+                                                 (int64_t)token * a.pool_stride[kind][1] +
+                                                 (int64_t)head * a.pool_stride[kind][2] + d);
+      scale = a.block_scales.scale[kind][(int64_t)page * a.block_scales.stride[kind][0] +
+                                   (int64_t)a.block_scales.by_block.div(token) * a.block_scales.stride[kind][1] +
+                                   (int64_t)head * a.block_scales.stride[kind][2]];
+    }
+    Pack<X, 8> x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float y = KV::load(in.v[j]) * scale;
+      asm("" : "+v"(y));  // the product in binary32 for every type (else one instruction rounds it to float16)
+      x.v[j] = X::store(y);
+    }
+    __builtin_memcpy(static_cast<typename X::Raw*>(a.out[kind]) + (int64_t)(t0 + t) * a.out_stride[kind][0] +
+                         (int64_t)head * a.out_stride[kind][1] + d, &x, sizeof x);
+  }
+}
+
+template <class X, class KV>
+hipError_t launch(BlockReadArgs a, hipStream_t s) {
+  const uint32_t row = a.dim / 8u, units = row * a.heads * ((a.out[0] != nullptr) + (a.out[1] != nullptr));
+  a.by_row = FastDiv::of(row);
+  a.by_token = FastDiv::of(units);
+  a.tokens_per_group = min(max(kThreads / units, 1u), kMaxTokens);
+  hipLaunchKernelGGL((block_read_kernel<X, KV>), dim3((a.T + a.tokens_per_group - 1u) / a.tokens_per_group), dim3(kThreads), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_kv_block_read(const BlockReadArgs& a, uint32_t dtype, uint32_t kv_dtype, hipStream_t s) {
+  const bool i8 = kv_dtype == LLMHIP_I8;
+  switch (dtype) {
+    case LLMHIP_F32: return i8 ? launch<F32, I8>(a, s) : launch<F32, E4M3>(a, s);
+    case LLMHIP_BF16: return i8 ? launch<BF16, I8>(a, s) : launch<BF16, E4M3>(a, s);
+    default: return i8 ? launch<F16, I8>(a, s) : launch<F16, E4M3>(a, s);
+  }
+}
+
+}  // namespace llmhip

@@ -21,6 +21,7 @@
 
 #include <type_traits>
 
+#include "kv_args.h"
 #include "kv_types.h"
 
 namespace llmhip {
@@ -95,17 +96,28 @@ __device__ __forceinline__ uint32_t finite2(T, uint32_t x) {
   const uint32_t low = (x & kTop) == kTop ? 0u : x & 0xffffu;
   return (x >> 16 & kTop) == kTop ? low : low | (x & 0xffff0000u);
 }
-// Two E4M3 values of a word as 16-bit values, exactly.
+// Two 8-bit values of a word as 16-bit values, exactly.
 template <bool HIGH>
-__device__ __forceinline__ uint32_t widen2(BF16, uint32_t x) {
+__device__ __forceinline__ uint32_t widen2(E4M3, BF16, uint32_t x) {
   return bits_as<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, HIGH));
 }
 template <bool HIGH>
-__device__ __forceinline__ uint32_t widen2(F16, uint32_t x) {
+__device__ __forceinline__ uint32_t widen2(E4M3, F16, uint32_t x) {
   return bits_as<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, HIGH));
 }
+// Whole numbers: by way of binary32.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t widen2(I8, BF16, uint32_t x) {
+  return pack2(BF16(), (float)(int8_t)(x >> (HIGH ? 16 : 0)), (float)(int8_t)(x >> (HIGH ? 24 : 8)));
+}
+// 1024 + (c + 128) is 0x6400 with c + 128 in its low byte.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t widen2(I8, F16, uint32_t x) {
+  const uint32_t y = __builtin_amdgcn_perm(0x64646464u, x ^ 0x80808080u, HIGH ? 0x04030402u : 0x04010400u);
+  return bits_as<uint32_t>(bits_as<f16x2>(y) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f});
+}
 
-// Queries of a 16-bit type over a cache of that type or E4M3. DIM: head_dim
+// Queries of a 16-bit type over a cache of that type or of 8 bits. DIM: head_dim
 // rounded up to one of 32, 64, 96, 128, 192 and 256; FULL: it is head_dim.
 // CHUNK: neighbouring values that a lane loads of a key, 16 in an E4M3 row
 // of whole 16s, else 8.
@@ -113,6 +125,9 @@ template <class Q_, class KV_, int DIM, bool FULL, int CHUNK>
 struct Engine16 {
   using Q = Q_;
   using KV = KV_;
+  using Args = AttendArgs;
+  static constexpr bool kBlocks = false;
+  static constexpr bool kLarge = false;  // more registers than two waves of a SIMD have
   static constexpr int kElem = sizeof(typename KV::Raw);
   static constexpr int kDim = DIM;
   static constexpr int kGroup = 8, kTile = 32, kProducts = 2;
@@ -122,9 +137,9 @@ struct Engine16 {
   // 8: no load or store passes the row's end.
   static constexpr int kVec = DIM == 32 ? 2 : DIM == 64 || (DIM == 192 && kElem == 2) ? 4 : 8;
   static constexpr int kPanels = (DIM + 16 * kVec - 1) / (16 * kVec);
-  // The numerators' and values' type in the second product. E4M3 values are
+  // The numerators' and values' type in the second product. 8-bit values are
   // exact in either; BF16 numerators have no smallest step to lose.
-  using W = std::conditional_t<std::is_same_v<KV, E4M3>, BF16, Q>;
+  using W = std::conditional_t<kElem == 1, BF16, Q>;
   // F16 has: numerators are held 2^kLift times as large, up to 2^15, and what
   // their rounding lost kSpread times as large again.
   static constexpr bool kNarrow = std::is_same_v<W, F16>;
@@ -199,10 +214,10 @@ struct Engine16 {
         for (int h = 0; h < kDeep; ++h) {
           u32x4 y;
           if constexpr (kElem == 1) {
-            y[0] = widen2<false>(Q(), k[a][t][2 * h]);
-            y[1] = widen2<true>(Q(), k[a][t][2 * h]);
-            y[2] = widen2<false>(Q(), k[a][t][2 * h + 1]);
-            y[3] = widen2<true>(Q(), k[a][t][2 * h + 1]);
+            y[0] = widen2<false>(KV(), Q(), k[a][t][2 * h]);
+            y[1] = widen2<true>(KV(), Q(), k[a][t][2 * h]);
+            y[2] = widen2<false>(KV(), Q(), k[a][t][2 * h + 1]);
+            y[3] = widen2<true>(KV(), Q(), k[a][t][2 * h + 1]);
           } else {
             y = k[a][t];
           }
@@ -259,7 +274,7 @@ struct Engine16 {
     uint32_t x;
     if constexpr (kVec * kElem <= 4) x = v[i][p];
     else x = v[i][p][kElem == 1 ? w >> 1 : w];
-    if constexpr (kElem == 1) return w & 1 ? widen2<true>(W(), x) : widen2<false>(W(), x);
+    if constexpr (kElem == 1) return w & 1 ? widen2<true>(KV(), W(), x) : widen2<false>(KV(), W(), x);
     else return x;
   }
 
@@ -311,12 +326,25 @@ struct Engine16 {
   }
 };
 
+// The same over a cache with a scale for each block of tokens and head, which
+// Run applies. EACH: blocks are no whole groups of tokens.
+template <class Q_, class KV_, int DIM, bool FULL, int CHUNK, bool EACH>
+struct BlockEngine : Engine16<Q_, KV_, DIM, FULL, CHUNK> {
+  using Args = BlockAttendArgs;
+  static constexpr bool kBlocks = true;
+  static constexpr bool kEach = EACH;
+  static constexpr bool kLarge = EACH && CHUNK == 8 && DIM > 64;
+};
+
 // Queries and cache in binary32: the products are 4 deep, one token of each
 // group and one value of each chunk at a time.
 template <int DIM, bool FULL>
 struct Engine32 {
   using Q = F32;
   using KV = F32;
+  using Args = AttendArgs;
+  static constexpr bool kBlocks = false;
+  static constexpr bool kLarge = false;
   static constexpr int kElem = 4;
   static constexpr int kDim = DIM;
   static constexpr int kGroup = 4, kTile = 16, kProducts = 1;

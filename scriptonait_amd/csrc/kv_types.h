@@ -39,6 +39,19 @@ struct E4M3 {
     return (Raw)(__builtin_amdgcn_cvt_pk_fp8_f32(x, 0.0f, 0, false) & 0xff);
   }
 };
+// Whole numbers; -128 is never stored. NaN is stored as 0.
+struct I8 {
+  using Raw = int8_t;
+  static constexpr uint32_t kId = LLMHIP_I8;
+  static constexpr float kMax = 127.0f;
+  __device__ static __forceinline__ float load(Raw x) { return (float)x; }
+  __device__ static __forceinline__ Raw store(float x) {
+    x = __builtin_rintf(x);
+    x = x > kMax ? kMax : x;
+    x = x < -kMax ? -kMax : x;
+    return (Raw)(int32_t)(x == x ? x : 0.0f);
+  }
+};
 
 // N values of one row, moved as one access.
 template <class T, int N>

@@ -7,6 +7,9 @@
              values and rotates queries, attend (llmhip_kv_attend) is the
              attention of one new token for each request
 
+kv_blocks.BlockKVCache is such a cache in 8 bits whose scales follow from what
+is written into it.
+
 All of them work on torch tensors on the device, are enqueued on `stream`
 (default: torch's current stream), allocate nothing and do not synchronize,
 so a whole step can be captured into a graph. With a `stream` of the caller's
@@ -31,7 +34,9 @@ from .sampler import Sampler, SamplerError, load_library
 KSTATUS_BAD_INDEX = 2
 F32, BF16, F16, E4M3 = 0, 1, 2, 3
 DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.float8_e4m3fn: E4M3}
-EXPORTED_SYMBOLS = ("llmhip_kv_plan", "llmhip_kv_append", "llmhip_kv_attend_workspace", "llmhip_kv_attend")
+EXPORTED_SYMBOLS = ("llmhip_kv_plan", "llmhip_kv_append", "llmhip_kv_attend_workspace", "llmhip_kv_attend",
+                    "llmhip_kv_block_append", "llmhip_kv_block_read", "llmhip_kv_block_attend_workspace",
+                    "llmhip_kv_block_attend")
 STYLES = {"halves": 0, "neighbours": 1}
 _NO_ROWS = (None, 0, 0)
 
@@ -46,6 +51,12 @@ class LlmhipKvCache(ctypes.Structure):
 
 class LlmhipRope(ctypes.Structure):
     _fields_ = [("freqs", _vp), ("dims", _u32), ("style", _u32)]
+
+
+class LlmhipKvBlocks(ctypes.Structure):
+    _fields_ = [("k_pool", _vp), ("v_pool", _vp), ("k_scale", _vp), ("v_scale", _vp), ("k_stride", _i64 * 3),
+                ("v_stride", _i64 * 3), ("k_scale_stride", _i64 * 3), ("v_scale_stride", _i64 * 3), ("dtype", _u32),
+                ("pages", _u32), ("page", _u32), ("block", _u32), ("heads", _u32), ("head_dim", _u32)]
 
 
 _lib: Optional[ctypes.CDLL] = None
@@ -67,6 +78,15 @@ def load_kv() -> ctypes.CDLL:
         lib.llmhip_kv_attend.restype = ctypes.c_int
         lib.llmhip_kv_attend.argtypes = [_vp, _vp, _u32, _sz, _sz, *rows, _vp, _sz, _sz, _vp, _sz, ctypes.c_float, *rows,
                                          _vp, _vp, _sz, _vp]
+        lib.llmhip_kv_block_append.restype = ctypes.c_int
+        lib.llmhip_kv_block_append.argtypes = lib.llmhip_kv_append.argtypes
+        lib.llmhip_kv_block_read.restype = ctypes.c_int
+        lib.llmhip_kv_block_read.argtypes = [_vp, _vp, _u32, _sz, _vp, *rows, *rows, _vp]
+        lib.llmhip_kv_block_attend_workspace.restype = ctypes.c_int
+        lib.llmhip_kv_block_attend_workspace.argtypes = [_vp, _vp, _sz, _sz, ctypes.POINTER(_sz)]
+        lib.llmhip_kv_block_attend.restype = ctypes.c_int
+        lib.llmhip_kv_block_attend.argtypes = [_vp, _vp, _u32, _sz, _sz, _sz, *rows, _i64, _vp, _sz, _sz, _vp, _sz,
+                                               ctypes.c_float, *rows, _i64, _vp, _vp, _sz, _vp]
         _lib = lib
     return _lib
 
