@@ -14,7 +14,10 @@ with everything on the device. Prompts go in one token a step, as the
 reference's prefill does (model.rs:311-322); requests end at their own
 lengths and give their pages back.
 
-  python examples/paged_decode.py [--dtype bf16|f16|f32|e4m3] [--steps N]
+With --dtype i8 the caches are of 8 bits with a scale for each block of tokens
+(BlockKVCache), which follow from what is written.
+
+  python examples/paged_decode.py [--dtype bf16|f16|f32|e4m3|i8] [--steps N]
 """
 from __future__ import annotations
 
@@ -29,6 +32,7 @@ import torch
 sys.path.insert(0, str(Path(__file__).resolve().parent.parent))
 
 from scriptonait_amd.kv import KVCache, PagePool, Rope  # noqa: E402
+from scriptonait_amd.kv_blocks import BlockKVCache  # noqa: E402
 from scriptonait_amd.sampler import Sampler, SamplingConfig  # noqa: E402
 
 
@@ -39,7 +43,8 @@ class Decoder:
                  context=96, page_size=16, pages=24, dtype="bf16", seed=0):
         dev = torch.device("cuda:0")
         g = torch.Generator().manual_seed(seed)
-        self.dtype = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32, "e4m3": torch.bfloat16}[dtype]
+        self.dtype = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32, "e4m3": torch.bfloat16,
+                      "i8": torch.bfloat16}[dtype]
         cached = torch.float8_e4m3fn if dtype == "e4m3" else self.dtype
         self.sampler, self.hidden, self.heads, self.kv_heads, self.window = sampler, hidden, heads, kv_heads, window
         self.dim = hidden // heads
@@ -51,8 +56,13 @@ class Decoder:
         self.pool = PagePool(sampler, pages, page_size)
         scales = [torch.full((kv_heads,), 0.02, device=dev) for _ in range(2)] if dtype == "e4m3" else []
         shape = (pages, page_size, kv_heads, self.dim)
-        self.caches = [KVCache(sampler, *[torch.zeros(shape, device=dev).to(cached) for _ in range(2)], *scales)
-                       for _ in range(layers)]
+        if dtype == "i8":
+            blocks = (pages, page_size // math.gcd(page_size, 16), kv_heads)
+            self.caches = [BlockKVCache(sampler, *[torch.zeros(shape, dtype=torch.int8, device=dev) for _ in range(2)],
+                                        *[torch.zeros(blocks, device=dev) for _ in range(2)]) for _ in range(layers)]
+        else:
+            self.caches = [KVCache(sampler, *[torch.zeros(shape, device=dev).to(cached) for _ in range(2)], *scales)
+                           for _ in range(layers)]
         self.workspace = self.caches[0].workspace(heads)
         i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)  # noqa: E731
         self.lens, self.granted, self.start = i32(batch), i32(batch), i32(batch + 1)
@@ -130,7 +140,7 @@ def generate(sampler, prompts, steps, config=None, seeds=None, on_step=None, mak
 
 def main():
     a = argparse.ArgumentParser(description=__doc__.splitlines()[0])
-    a.add_argument("--dtype", choices=["bf16", "f16", "f32", "e4m3"], default="bf16")
+    a.add_argument("--dtype", choices=["bf16", "f16", "f32", "e4m3", "i8"], default="bf16")
     a.add_argument("--steps", type=int, default=64)
     args = a.parse_args()
     prompts = [([1, 2, 3], args.steps), ([10, 11, 12, 13, 14], args.steps // 2), ([7], args.steps), ([5, 6], args.steps * 3 // 4)]
