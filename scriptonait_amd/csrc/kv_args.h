@@ -59,10 +59,10 @@ struct BlockScales {
 
 struct BlockAppendArgs : AppendArgs {
   BlockScales block_scales;
-  uint32_t kv_groups, kv_parts;  // workgroups of the keys and values: groups of tokens, and workgroups for each
-  uint32_t kv_tokens;            // tokens of such a group
-  uint32_t kv_waves;             // heads of such a workgroup
-  uint32_t turn_tokens;          // tokens whose cosines and sines LDS holds
+  uint32_t kv_tokens, kv_groups, kv_parts;  // groups of tokens whose keys and values are written, and workgroups for each
+  uint32_t turn_tokens;                     // tokens whose cosines and sines LDS holds
+  bool short_slots;              // the pool has less than 2^31 tokens
+  FastDiv by_half, by_heads, by_page;
 };
 
 struct BlockReadArgs {
@@ -73,7 +73,8 @@ struct BlockReadArgs {
   BlockScales block_scales;
   const int64_t* slots;
   uint32_t T, heads, dim, pages, page;
-  FastDiv by_token, by_row;  // units of a token, units of a head row
+  bool short_slots;  // the pool has less than 2^31 tokens
+  FastDiv by_token, by_row, by_page;  // units of a token, units of a head row
   uint32_t tokens_per_group;
   uint32_t* status;
 };

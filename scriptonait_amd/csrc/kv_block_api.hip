@@ -12,7 +12,6 @@ namespace {
 
 constexpr uint32_t kMaxBlock = 256;
 constexpr size_t kMaxNewTokens = 16;
-constexpr uint64_t kMaxThreads = 0xffffffffu;  // of a launch
 
 int check_blocks(const llmhip_kv_blocks* c) {
   ARG(c, "cache is null");
@@ -101,9 +100,6 @@ int llmhip_kv_block_append(llmhip_ctx* ctx, const llmhip_kv_blocks* cache, uint3
   const uint32_t least = 8 / elem;
   while (vec >= least && (dims % (2 * vec) || (dim - dims) % (2 * vec))) vec /= 2;
   if (vec < least) vec = 1;
-  // At most T groups of tokens of keys and values, of up to 8 heads each, and T of queries.
-  const uint64_t groups = (uint64_t)T * (2 * ((cache->heads + 7) / 8) / (T >= 16384 ? 16.0 : 1.0) + 2.0);
-  SUPPORTED(groups * 512 <= kMaxThreads, "T times heads too large");
   ON_DEVICE(info);
   BlockAppendArgs a{};
   a.x[0] = q;

@@ -2,15 +2,16 @@
 // rotated (llmhip_kv_block_append).
 //
 // A block's scale needs the largest of its new values before the first code
-// can be written. A wave takes one head of one block's new tokens, keys or
-// values: it holds what it has read (and turned) in registers while the
-// maximum goes across its lanes, then writes codes; of more than it can hold
-// it reads the rest again, from the L2. So a value comes from memory once and
-// blocks need no workgroup-wide step but the cosines and sines, which all heads
-// of a workgroup share in LDS. Kept tokens are read only where the scale grew.
-// Units are laid out as in the append to a cache of values: 2 * VEC values of
-// a row, VEC pairs, or values that are not rotated.
-#include <type_traits>
+// can be written. A workgroup finds the blocks that begin among 16 tokens (their
+// slots say so) and gives each block and head as many neighbouring lanes as
+// hold all of its new values in registers: 8 for a decoding request's single row
+// of 128 values, all 256 for 64 of them. The maximum goes across those lanes, and
+// codes are written. Of blocks that are larger the rows are read again, from
+// the L2. So a value comes from memory once. Cosines and sines are computed
+// once for all heads of a workgroup, into LDS. Kept tokens are read only where
+// the scale grew. Units are laid out as in the append to a cache of values: 2 *
+// VEC values of a row, VEC pairs, or values that are not rotated.
+#include <algorithm>
 
 #include "kv_args.h"
 #include "kv_turn.h"
@@ -20,9 +21,13 @@
 namespace llmhip {
 namespace {
 
-constexpr uint32_t kMaxWaves = 8;
-constexpr uint32_t kMaxTokens = 8;      // of a workgroup of queries
-constexpr uint32_t kMaxTurns = 4096;    // cosines and sines in LDS: 32 KiB
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kMaxTokens = 8;  // of a workgroup of queries
+constexpr uint32_t kMaxGroup = 64;  // of one of keys or values: a lane's each
+
+// Units of a lane in registers: 32 values, 16 where they take more addresses.
+template <int VEC>
+constexpr uint32_t kHeld = VEC >= 4 ? 16 / VEC : 8 / VEC;
 
 template <int BYTES>
 struct Word;
@@ -64,22 +69,27 @@ __device__ __forceinline__ Unit unit_of(uint32_t c, uint32_t dims, uint32_t dim)
   return {d0, d0 + (NEIGHBOURS ? VEC : apart), turned};
 }
 
-// The unit's values in binary32; turn: its token's cosines and sines.
+// The unit's values as they are stored, of which the first and the second half
+// are its two vectors.
 template <class X, int VEC, bool NEIGHBOURS>
-__device__ __forceinline__ void get(float* x, const typename X::Raw* row, const Unit& u, uint32_t c, const float2* turn) {
+__device__ __forceinline__ Pack<X, 2 * VEC> get(const typename X::Raw* row, const Unit& u) {
   if constexpr (NEIGHBOURS && VEC > 1) {
-    const Pack<X, 2 * VEC> in = load_pack<X, 2 * VEC>(row + u.d0);
-#pragma unroll
-    for (int j = 0; j < 2 * VEC; ++j) x[j] = X::load(in.v[j]);
+    return load_pack<X, 2 * VEC>(row + u.d0);
   } else {
     const Pack<X, VEC> p0 = load_pack<X, VEC>(row + u.d0), p1 = load_pack<X, VEC>(row + u.d1);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      x[j] = X::load(p0.v[j]);
-      x[VEC + j] = X::load(p1.v[j]);
-    }
+    Pack<X, 2 * VEC> x;
+    __builtin_memcpy(x.v, &p0, sizeof p0);
+    __builtin_memcpy(x.v + VEC, &p1, sizeof p1);
+    return x;
   }
-  if (u.turned) {
+}
+
+// In binary32 and rotated; turn: its token's cosines and sines.
+template <class X, int VEC, bool NEIGHBOURS>
+__device__ __forceinline__ void rotate(float* x, const Pack<X, 2 * VEC>& in, bool turned, uint32_t c, const float2* turn) {
+#pragma unroll
+  for (int j = 0; j < 2 * VEC; ++j) x[j] = X::load(in.v[j]);
+  if (turned) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
       const int ia = NEIGHBOURS ? 2 * j : j, ib = NEIGHBOURS ? 2 * j + 1 : VEC + j;
@@ -111,203 +121,329 @@ __device__ __forceinline__ void put(typename T::Raw* row, const Unit& u, const f
   }
 }
 
-// The largest finite magnitude (fmax drops the NaN that it meets).
+// Codes of numbers that are finite and at most MAX (and 2^-22 of it), two or
+// four at a time: whole numbers are the low byte of 1.5 * 2^23 and the number.
+__device__ __forceinline__ uint32_t codes4(I8, float x0, float x1, float x2, float x3) {
+  constexpr float kMagic = 12582912.0f;
+  const uint32_t lo = __builtin_amdgcn_perm(__float_as_uint(x1 + kMagic), __float_as_uint(x0 + kMagic), 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(__float_as_uint(x3 + kMagic), __float_as_uint(x2 + kMagic), 0x0c0c0400u);
+  return lo | hi << 16;
+}
+__device__ __forceinline__ uint32_t codes4(E4M3, float x0, float x1, float x2, float x3) {
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x2, x3, __builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false), true);
+}
+template <class KV, int VEC, bool NEIGHBOURS>
+__device__ __forceinline__ void put_finite(typename KV::Raw* row, const Unit& u, const float* x, float r) {
+  if constexpr (VEC == 1) {
+    put<KV, VEC, NEIGHBOURS>(row, u, x, r);
+  } else {
+    uint32_t w[(VEC + 1) / 2];
+#pragma unroll
+    for (int j = 0; j < 2 * VEC; j += 4) w[j / 4] = codes4(KV(), x[j] * r, x[j + 1] * r, x[j + 2] * r, x[j + 3] * r);
+    constexpr int kBytes = NEIGHBOURS ? 2 * VEC : VEC;
+    Pack<KV, kBytes> p;
+    __builtin_memcpy(p.v, w, kBytes);
+    store_once<KV, kBytes>(row + u.d0, p);
+    if constexpr (!NEIGHBOURS) {
+      __builtin_memcpy(p.v, reinterpret_cast<const char*>(w) + VEC, VEC);
+      store_once<KV, VEC>(row + u.d1, p);
+    }
+  }
+}
+
+// Magnitudes in an order that has infinities and NaN below all numbers: the
+// bits without the sign, plus what makes those of infinity wrap to 0.
 template <int N>
-__device__ __forceinline__ float largest(float top, const float* x) {
+__device__ __forceinline__ void range_of(uint32_t& top, uint32_t& low, const float* x) {
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const float y = __builtin_fabsf(x[j]);
-    top = __builtin_fmaxf(top, y == INFINITY ? 0.0f : y);
+    const uint32_t y = (__float_as_uint(x[j]) << 1) + 0x01000000u;
+    top = max(top, y);
+    low = min(low, y);
   }
-  return top;
+}
+__device__ __forceinline__ float magnitude(uint32_t top) {
+  return top < 0x01000000u ? 0.0f : __uint_as_float((top - 0x01000000u) >> 1);
 }
 
+// Cosines and sines of n tokens from t0 on. A thread takes every few tokens of
+// one pair; while positions go on as tokens do, the next turn is the one before
+// and a step's: four products and not two series, each of which adds no more
+// than 2^-51 (the 80 steps that LDS holds, 2^-44).
 __device__ __forceinline__ void fill_turns(float2* turns, const BlockAppendArgs& a, uint32_t t0, uint32_t n) {
-  const uint32_t half = a.dims / 2u;
-  for (uint32_t i = threadIdx.x; i < n * half; i += blockDim.x) {
-    const uint32_t t = i / half;
-    turns[i] = cos_sin((double)a.positions[t0 + t] * a.freqs[i - t * half]);
+  const uint32_t half = a.by_half.d, first = a.by_half.div(threadIdx.x), pair = threadIdx.x - first * half;
+  const uint32_t stride = a.by_half.div(kThreads);
+  if (first >= min(stride, n)) return;
+  const double freq = a.freqs[pair];
+  const bool many = first + stride < n;
+  const Turn step = many ? turn_of<true>((double)stride * freq) : Turn{1.0, 0.0};
+  Turn now = {1.0, 0.0};
+  int32_t at = a.positions[t0 + first], next = at;
+  int64_t expected = (int64_t)at + 1;  // of the first: no turn before it
+#pragma unroll 1
+  for (uint32_t i = first; i < n; i += stride, at = next) {
+    if (i + stride < n) next = a.positions[t0 + i + stride];
+    if (at == expected) now = Turn{now.cos * step.cos - now.sin * step.sin, now.cos * step.sin + now.sin * step.cos};
+    else now = turn_of<true>((double)at * freq);
+    expected = (int64_t)at + stride;
+    turns[i * half + pair] = {(float)now.cos, (float)now.sin};
   }
 }
 
-// The n new tokens t0 .. of one block, first of them at place `token` of page
-// `page`: one head's keys (KIND 0) or values (KIND 1). All waves of the
-// workgroup come here together; one that is not `live` has no head.
-template <class X, class KV, int VEC, bool NEIGHBOURS>
-__device__ __forceinline__ void write_block(const BlockAppendArgs& a, float2* turns, int kind, uint32_t head, bool live,
-                                            uint32_t t0, uint32_t n, uint32_t page, uint32_t token) {
-  constexpr uint32_t kHeld = VEC == 1 ? 8 : 64 / (2 * VEC);  // units of a lane in registers
-  const uint32_t lane = lane_id(), row = a.by_row.d;
-  const uint32_t dims = kind ? 0u : a.dims, half = dims / 2u;
-  const uint32_t chunk = dims ? a.turn_tokens : n;  // tokens whose cosines and sines are there
-  const uint32_t block = a.block_scales.by_block.div(token), place = token - block * a.block_scales.by_block.d;
-  const typename X::Raw* in = static_cast<const typename X::Raw*>(a.x[1 + kind]) + (int64_t)t0 * a.x_stride[1 + kind][0] +
-                              (int64_t)head * a.x_stride[1 + kind][1];
-  typename KV::Raw* out = static_cast<typename KV::Raw*>(a.pool[kind]) + (int64_t)page * a.pool_stride[kind][0] +
-                          (int64_t)token * a.pool_stride[kind][1] + (int64_t)head * a.pool_stride[kind][2];
-  float* scale = a.block_scales.scale[kind] + (int64_t)page * a.block_scales.stride[kind][0] +
-                 (int64_t)block * a.block_scales.stride[kind][1] + (int64_t)head * a.block_scales.stride[kind][2];
-  const float old = live && place ? *scale : 0.0f;
+// New tokens that stand next to each other in one block.
+struct Run {
+  uint32_t t0, n;        // first token of the batch, and how many
+  uint32_t page, token;  // where the first one goes
+};
 
-  float held[kHeld][2 * VEC], top = 0.0f;
-  const auto each = [&](uint32_t u, float* x, uint32_t c0, auto&& use) {
-    const uint32_t t = a.by_row.div(u), c = u - t * row;
-    const Unit at = unit_of<VEC, NEIGHBOURS>(c, dims, a.dim);
-    get<X, VEC, NEIGHBOURS>(x, in + (int64_t)(c0 + t) * a.x_stride[1 + kind][0], at, c, turns + t * half);
-    use(at, c0 + t);
-  };
-  for (uint32_t c0 = 0; c0 < n; c0 += chunk) {
-    const uint32_t units = live ? min(chunk, n - c0) * row : 0u;
-    if (dims) {
-      __syncthreads();  // (the ones before are used)
-      fill_turns(turns, a, t0 + c0, min(chunk, n - c0));
-      __syncthreads();
-    }
-    if (n <= chunk) {
-#pragma unroll
-      for (uint32_t k = 0; k < kHeld; ++k) {
-#pragma unroll
-        for (int j = 0; j < 2 * VEC; ++j) held[k][j] = 0.0f;
-        if (lane + 64u * k < units) each(lane + 64u * k, held[k], c0, [](const Unit&, uint32_t) {});
-      }
-#pragma unroll
-      for (uint32_t k = 0; k < kHeld; ++k) top = largest<2 * VEC>(top, held[k]);
-    }
-    for (uint32_t u = lane + (n <= chunk ? 64u * kHeld : 0u); u < units; u += 64u) {
-      float x[2 * VEC];
-      each(u, x, c0, [](const Unit&, uint32_t) {});
-      top = largest<2 * VEC>(top, x);
-    }
-  }
-#pragma unroll
-  for (uint32_t off = 32; off > 0; off >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, off, 64));
-  float s = top / KV::kMax;
-  s = s < 0x1p-126f ? 0.0f : s;
-  s = old > s ? old : s;
-  const float r = s > 0.0f ? 1.0f / s : 1.0f;  // (1: all finite values are so small that they round to 0)
-  if (live && lane == 0u && !(s == old && place)) *scale = s;
-  if (live && place && s > old) {  // kept tokens: 8 codes at a time
-    const float f = old / s;
-    const uint32_t eights = a.dim / 8u;
-    typename KV::Raw* first = out - (int64_t)place * a.pool_stride[kind][1];
-    for (uint32_t u = lane; u < place * eights; u += 64u) {
-      const uint32_t t = u / eights;
-      typename KV::Raw* p = first + (int64_t)t * a.pool_stride[kind][1] + (u - t * eights) * 8u;
-      Pack<KV, 8> x = *reinterpret_cast<const Pack<KV, 8>*>(p);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x.v[j] = KV::store(KV::load(x.v[j]) * f);
-      *reinterpret_cast<Pack<KV, 8>*>(p) = x;
-    }
-  }
-  for (uint32_t c0 = 0; c0 < n; c0 += chunk) {
-    const uint32_t units = live ? min(chunk, n - c0) * row : 0u;
-    if (n <= chunk) {
-#pragma unroll
-      for (uint32_t k = 0; k < kHeld; ++k) {
-        const uint32_t u = lane + 64u * k, t = a.by_row.div(u);
-        if (u < units)
-          put<KV, VEC, NEIGHBOURS>(out + (int64_t)t * a.pool_stride[kind][1], unit_of<VEC, NEIGHBOURS>(u - t * row, dims, a.dim), held[k], r);
-      }
-    } else if (dims) {
-      __syncthreads();
-      fill_turns(turns, a, t0 + c0, min(chunk, n - c0));
-      __syncthreads();
-    }
-    for (uint32_t u = lane + (n <= chunk ? 64u * kHeld : 0u); u < units; u += 64u) {
-      float x[2 * VEC];
-      each(u, x, c0, [&](const Unit& at, uint32_t t) {
-        put<KV, VEC, NEIGHBOURS>(out + (int64_t)t * a.pool_stride[kind][1], at, x, r);
-      });
-    }
-  }
-}
-
+// The keys (KIND 0) or values (KIND 1) of the blocks that begin in a group of
+// tokens (or go on there with a token that is no neighbour of the one before).
 template <class X, class KV, int VEC, bool NEIGHBOURS>
-__global__ __launch_bounds__(kMaxWaves * 64) void block_append_kernel(BlockAppendArgs a) {
-  extern __shared__ float2 s_turn[];
+__device__ __forceinline__ void write_blocks(const BlockAppendArgs& a, float2* turns, uint32_t group, int kind, uint32_t part) {
+  constexpr uint32_t kHold = kHeld<VEC>;
+  __shared__ Run s_run[kMaxGroup];
+  __shared__ uint32_t s_top[kThreads / 64];
   const uint32_t tid = threadIdx.x, lane = lane_id(), wave = readlane_u32(tid >> 6, 0);
-  if (blockIdx.x < a.kv_groups * a.kv_parts) {
-    // Keys or values of kv_waves heads, of the blocks that begin in a group of
-    // tokens (or go on there with a token that is no neighbour of the last).
-    const uint32_t group = blockIdx.x / a.kv_parts, part = blockIdx.x - group * a.kv_parts;
-    const int kind = part >= a.kv_parts / 2u;
-    const uint32_t head = (part - kind * (a.kv_parts / 2u)) * a.kv_waves + wave;
-    const uint32_t t = group * a.kv_tokens + lane;
-    const int64_t slot = lane < a.kv_tokens && t < a.T ? a.slots[t] : -1;
-    uint32_t page = 0, token = 0;
-    bool bad = false, first = split_slot(slot, a.pages, a.page, page, token, bad);
-    if (bad && part == 0u && wave == 0u) atomicOr(a.status, LLMHIP_KSTATUS_BAD_INDEX);
-    const uint32_t place = a.block_scales.by_block.mod(token);
-    if (first && place && t) first = a.slots[t - 1u] != slot - 1;
-    for (uint64_t runs = __ballot(first); runs; runs &= runs - 1u) {
-      const uint32_t at = (uint32_t)__builtin_ctzll(runs);
-      const uint32_t t0 = readlane_u32(t, at);
-      const int64_t slot0 = (int64_t)readlane_u64((uint64_t)slot, at);
-      const uint32_t most = min(a.block_scales.by_block.d - readlane_u32(place, at), a.T - t0);
-      uint32_t n = 0;
-      while (n < most) {
-        const uint32_t i = n + lane;
-        const uint64_t other = ~__ballot(i < most && a.slots[t0 + i] == slot0 + i);
-        n += other ? (uint32_t)__builtin_ctzll(other) : 64u;
-        if (other) break;
-      }
-      write_block<X, KV, VEC, NEIGHBOURS>(a, s_turn, kind, min(head, a.heads - 1u), head < a.heads, t0, n, readlane_u32(page, at),
-                                          readlane_u32(token, at));
+  const uint32_t begin = group * a.kv_tokens, size = min(a.kv_tokens, a.T - begin), t = begin + lane;
+
+  // The runs, which every wave finds for itself.
+  const int64_t slot = lane < size ? a.slots[t] : -1, before = lane < size && t ? a.slots[t - 1u] : -2;
+  uint32_t page = 0, token = 0;
+  bool bad = false;
+  const bool live_slot = a.short_slots ? split_short_slot(slot, a.pages, a.by_page, page, token, bad)
+                                       : split_slot(slot, a.pages, a.page, page, token, bad);
+  if (bad && part == 0u && kind == 0 && wave == 0u) atomicOr(a.status, LLMHIP_KSTATUS_BAD_INDEX);
+  const uint32_t block_size = a.block_scales.by_block.d, in_block = a.block_scales.by_block.mod(token);
+  const bool goes_on = live_slot && in_block && before == slot - 1;
+  const uint64_t first = __ballot(live_slot && !goes_on), others = __ballot(goes_on);
+  const uint32_t runs = (uint32_t)__builtin_popcountll(first);
+  if (!runs) return;
+  const uint64_t behind = ~(others >> 1 >> lane);  // (the top bit is always set)
+  uint32_t n = 1u + (uint32_t)__builtin_ctzll(behind);
+  const uint32_t last = 63u - (uint32_t)__builtin_clzll(first);
+  if (last + readlane_u32(n, last) == size) {  // the last one may go on behind the group
+    const int64_t slot0 = (int64_t)readlane_u64((uint64_t)slot, last);
+    const uint32_t most = min(block_size - readlane_u32(in_block, last), a.T - begin - last);
+    uint32_t has = size - last;
+    while (has < most) {
+      const uint32_t i = has + lane;
+      const uint64_t other = ~__ballot(i < most && a.slots[begin + last + min(i, most - 1u)] == slot0 + i);
+      has += other ? (uint32_t)__builtin_ctzll(other) : 64u;
+      if (other) break;
     }
+    n = lane == last ? has : n;
+  }
+  const bool leads = first >> lane & 1u;
+  uint32_t most_tokens = leads ? n : 0u;
+#pragma unroll
+  for (uint32_t off = 1; off < kMaxGroup; off *= 2u) most_tokens = max(most_tokens, (uint32_t)__shfl_xor((int)most_tokens, (int)off, 64));
+  most_tokens = readlane_u32(most_tokens, 0);
+  if (wave == 0u && leads) s_run[lanes_below(first)] = Run{t, n, page, token};
+  __syncthreads();
+
+  // A block's head is a task of `lanes` lanes.
+  const uint32_t row = a.by_row.d, dims = kind ? 0u : a.dims, half = dims / 2u;
+  const uint32_t longest = most_tokens * row, share = max((longest + kHold - 1u) / kHold, min(row, longest));
+  const uint32_t log_lanes = share >= kThreads ? 8u : share <= 1u ? 0u : 32u - (uint32_t)__builtin_clz(share - 1u);
+  const uint32_t lanes = 1u << log_lanes, at_once = kThreads >> log_lanes, tasks = runs * a.heads;
+  const uint32_t step = lanes * kHold, steps = (longest + step - 1u) / step;  // units at a time; more than one: all lanes' task
+  uint32_t turns_from = 0u, turns_to = 0u;  // tokens whose cosines and sines are there
+  const auto run_of = [&](uint32_t task) { return a.by_heads.div(task); };
+  for (uint32_t turn = part, task0 = turn * at_once, stop; task0 < tasks;
+       task0 = stop < min((turn + 1u) * at_once, tasks) ? stop : (turn += a.kv_parts) * at_once) {
+    // Tasks task0 .. stop, whose runs' tokens fit the table of cosines and sines.
+    stop = min((turn + 1u) * at_once, tasks);
+    const uint32_t run0 = run_of(task0), from = s_run[run0].t0;
+    uint32_t run1 = run_of(stop - 1u), upto = s_run[run1].t0 + s_run[run1].n;
+    while (half && steps == 1u && upto - from > a.turn_tokens && run1 > run0) {
+      stop = run1 * a.heads;
+      --run1;
+      upto = s_run[run1].t0 + s_run[run1].n;
+    }
+    const uint32_t task = task0 + (tid >> log_lanes), me = tid & (lanes - 1u);
+    const bool live = task < stop;
+    const uint32_t mine = min(task, stop - 1u), r = run_of(mine), head = mine - r * a.heads;
+    const Run run = s_run[r];
+    const uint32_t units = live ? run.n * row : 0u;
+
+    const uint32_t block = a.block_scales.by_block.div(run.token), place = run.token - block * block_size;
+    const typename X::Raw* in = static_cast<const typename X::Raw*>(a.x[1 + kind]) + (int64_t)run.t0 * a.x_stride[1 + kind][0] +
+                                (int64_t)head * a.x_stride[1 + kind][1];
+    typename KV::Raw* out = static_cast<typename KV::Raw*>(a.pool[kind]) + (int64_t)run.page * a.pool_stride[kind][0] +
+                            (int64_t)run.token * a.pool_stride[kind][1] + (int64_t)head * a.pool_stride[kind][2];
+    float* scale = a.block_scales.scale[kind] + (int64_t)run.page * a.block_scales.stride[kind][0] +
+                   (int64_t)block * a.block_scales.stride[kind][1] + (int64_t)head * a.block_scales.stride[kind][2];
+    const float old = live && place ? *scale : 0.0f;
+
+    // The task's units in steps of as many as its lanes hold: read and looked at,
+    // then written; of more than one step all are read again.
+    float x[kHold][2 * VEC];
+    uint32_t top = 0u, low = ~0u;
+    float by = 1.0f;
+#pragma unroll 1
+    for (uint32_t p = 0; p < 2u * steps; ++p) {
+      const bool writes = p >= steps;
+      const uint32_t first_unit = (writes ? p - steps : p) * step + me;
+      if (!writes || steps > 1u) {
+        Pack<X, 2 * VEC> raw[kHold];
+#pragma unroll
+        for (uint32_t k = 0; k < kHold; ++k) {
+          const uint32_t u = first_unit + k * lanes, i = a.by_row.div(u);
+          raw[k] = Pack<X, 2 * VEC>{};
+          if (u < units)
+            raw[k] = get<X, VEC, NEIGHBOURS>(in + (int64_t)i * a.x_stride[1 + kind][0], unit_of<VEC, NEIGHBOURS>(u - i * row, dims, a.dim));
+        }
+        // Cosines and sines of the step's tokens, from turned_from on.
+        uint32_t turned_from = from;
+        if (half) {
+          uint32_t to = upto;
+          if (steps > 1u) {
+            const uint32_t unit0 = first_unit - me;
+            turned_from += a.by_row.div(unit0);
+            to = min(upto, from + a.by_row.div(unit0 + step - 1u) + 1u);
+          }
+          if (turned_from != turns_from || to != turns_to) {
+            __syncthreads();  // (the ones before are used)
+            fill_turns(turns, a, turned_from, to > turned_from ? to - turned_from : 0u);  // (a shorter run has none in the last steps)
+            __syncthreads();
+            turns_from = turned_from;
+            turns_to = to;
+          }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kHold; ++k) {
+          const uint32_t u = first_unit + k * lanes, i = a.by_row.div(u), c = u - i * row;
+          rotate<X, VEC, NEIGHBOURS>(x[k], raw[k], u < units && c * 2u * VEC < dims, c, turns + (run.t0 + i - turned_from) * half);
+          range_of<2 * VEC>(top, low, x[k]);
+        }
+      }
+      if (p + 1u == steps) {
+        for (uint32_t off = 1; off < min(lanes, 64u); off *= 2u) top = max(top, (uint32_t)__shfl_xor((int)top, (int)off, 64));
+        if (lanes > 64u) {
+          __syncthreads();
+          if (lane == 0u) s_top[wave] = top;
+          __syncthreads();
+          for (uint32_t w = 0; w < lanes / 64u; ++w) top = max(top, s_top[(wave & ~(lanes / 64u - 1u)) + w]);
+        }
+        float s = magnitude(top) / KV::kMax;
+        s = s < 0x1p-126f ? 0.0f : s;
+        s = old > s ? old : s;
+        by = s > 0.0f ? 1.0f / s : 1.0f;  // (1: all finite values are so small that they round to 0)
+        if (live && me == 0u && !(place && s == old)) *scale = s;
+        if (live && place && s > old) {  // kept tokens: 8 codes at a time
+          const float f = old / s;
+          const uint32_t eights = a.dim / 8u;
+          typename KV::Raw* kept = out - (int64_t)place * a.pool_stride[kind][1];
+          for (uint32_t u = me; u < place * eights; u += lanes) {
+            const uint32_t i = u / eights;
+            typename KV::Raw* c = kept + (int64_t)i * a.pool_stride[kind][1] + (u - i * eights) * 8u;
+            Pack<KV, 8> codes = *reinterpret_cast<const Pack<KV, 8>*>(c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) codes.v[j] = KV::store(KV::load(codes.v[j]) * f);
+            *reinterpret_cast<Pack<KV, 8>*>(c) = codes;
+          }
+        }
+      }
+      if (writes) {
+        const bool odd = __any(low < 0x01000000u);
+#pragma unroll
+        for (uint32_t k = 0; k < kHold; ++k) {
+          const uint32_t u = first_unit + k * lanes, i = a.by_row.div(u);
+          if (u >= units) continue;
+          const Unit at = unit_of<VEC, NEIGHBOURS>(u - i * row, dims, a.dim);
+          typename KV::Raw* to = out + (int64_t)i * a.pool_stride[kind][1];
+          if (__builtin_expect(odd, 0)) put<KV, VEC, NEIGHBOURS>(to, at, x[k], by);
+          else put_finite<KV, VEC, NEIGHBOURS>(to, at, x[k], by);
+        }
+      }
+    }
+  }
+}
+
+template <class X, class KV, int VEC, bool NEIGHBOURS>
+__global__ __launch_bounds__(kThreads, 4) void block_append_kernel(BlockAppendArgs a) {
+  extern __shared__ float2 s_turn[];
+  const uint32_t tid = threadIdx.x;
+  // (Keys and values first: spread among the queries' workgroups they end later,
+  // 16384 tokens 95 us, not 90.)
+  const uint32_t kv = a.kv_groups * 2u * a.kv_parts;
+  if (blockIdx.x < kv) {
+    const uint32_t group = blockIdx.x / (2u * a.kv_parts), part = blockIdx.x - group * 2u * a.kv_parts;
+    write_blocks<X, KV, VEC, NEIGHBOURS>(a, s_turn, group, part & 1u, part >> 1);
     return;
   }
-  const uint32_t t0 = (blockIdx.x - a.kv_groups * a.kv_parts) * a.tokens_per_group, n = min(a.tokens_per_group, a.T - t0);
-  if (a.dims) {
+  const uint32_t t0 = (blockIdx.x - kv) * a.tokens_per_group, n = min(a.tokens_per_group, a.T - t0);
+  const uint32_t half = a.dims / 2u, units = n * a.by_token.d;
+  // A thread's first unit is on its way while the cosines and sines are computed.
+  const auto unit_at = [&](uint32_t u, uint32_t& t, uint32_t& head, uint32_t& c) {
+    t = a.by_token.div(u);
+    const uint32_t in_token = u - t * a.by_token.d;
+    head = a.by_row.div(in_token);
+    c = in_token - head * a.by_row.d;
+  };
+  const auto row_of = [&](uint32_t t, uint32_t head) {
+    return static_cast<const typename X::Raw*>(a.x[0]) + (int64_t)(t0 + t) * a.x_stride[0][0] + (int64_t)head * a.x_stride[0][1];
+  };
+  uint32_t t, head, c;
+  unit_at(min(tid, units - 1u), t, head, c);
+  Pack<X, 2 * VEC> in = get<X, VEC, NEIGHBOURS>(row_of(t, head), unit_of<VEC, NEIGHBOURS>(c, a.dims, a.dim));
+  if (half) {
     fill_turns(s_turn, a, t0, n);
     __syncthreads();
   }
-  const uint32_t half = a.dims / 2u;
-  for (uint32_t u = tid; u < n * a.by_token.d; u += blockDim.x) {
-    const uint32_t t = a.by_token.div(u), in_token = u - t * a.by_token.d;
-    const uint32_t head = a.by_row.div(in_token), c = in_token - head * a.by_row.d;
+#pragma unroll 1
+  for (uint32_t u = tid; u < units; u += kThreads) {
+    if (u != tid) {
+      unit_at(u, t, head, c);
+      in = get<X, VEC, NEIGHBOURS>(row_of(t, head), unit_of<VEC, NEIGHBOURS>(c, a.dims, a.dim));
+    }
     const Unit at = unit_of<VEC, NEIGHBOURS>(c, a.dims, a.dim);
     float x[2 * VEC];
-    get<X, VEC, NEIGHBOURS>(x, static_cast<const typename X::Raw*>(a.x[0]) + (int64_t)(t0 + t) * a.x_stride[0][0] +
-                                   (int64_t)head * a.x_stride[0][1], at, c, s_turn + t * half);
+    rotate<X, VEC, NEIGHBOURS>(x, in, at.turned, c, s_turn + t * half);
     put<X, VEC, NEIGHBOURS>(static_cast<typename X::Raw*>(a.out_q) + (int64_t)(t0 + t) * a.oq_stride[0] +
                                 (int64_t)head * a.oq_stride[1], at, x, 1.0f);
   }
 }
 
-template <class X, class KV>
-hipError_t launch(BlockAppendArgs a, bool neighbours, uint32_t vec, hipStream_t s) {
-  a.kv_waves = min(a.heads, kMaxWaves);
-  const uint32_t threads = a.kv_waves * 64u, row = a.dim / (2u * vec), units = row * a.q_heads;
+template <class X, class KV, int VEC, bool NEIGHBOURS>
+hipError_t launch_vec(BlockAppendArgs a, hipStream_t s) {
+  const uint32_t row = a.dim / (2u * VEC), units = row * a.q_heads, half = a.dims / 2u, block = a.block_scales.by_block.d;
   a.by_row = FastDiv::of(row);
   a.by_token = FastDiv::of(units ? units : 1u);
-  // A token of a group where few are (a decode step's are blocks of their
-  // own), up to 16, the more of which are one block's, of prompts.
-  a.kv_tokens = min(max(a.T / 1024u, 1u), 16u);
+  a.by_half = FastDiv::of(half ? half : 1u);
+  a.by_heads = FastDiv::of(a.heads);
+  a.by_page = FastDiv::of(a.page);
+  a.short_slots = (uint64_t)a.pages * a.page <= 0x7fffffffu;
+  a.tokens_per_group = units ? std::min(std::max(kThreads / units, 1u), kMaxTokens) : 1u;
+  // About the tokens of a block, so that a workgroup seldom finds none that begins.
+  a.kv_tokens = std::min(std::max(block, 16u), kMaxGroup);
   a.kv_groups = (a.T + a.kv_tokens - 1u) / a.kv_tokens;
-  a.kv_parts = 2u * ((a.heads + a.kv_waves - 1u) / a.kv_waves);
-  a.tokens_per_group = units ? min(max(threads / units, 1u), kMaxTokens) : 1u;
-  const uint32_t half = a.dims / 2u;
-  a.turn_tokens = half ? min(a.block_scales.by_block.d, kMaxTurns / half) : 1u;
-  const uint32_t lds = half * max(a.turn_tokens, a.tokens_per_group) * (uint32_t)sizeof(float2);
-  const dim3 grid(a.kv_groups * a.kv_parts + (units ? (a.T + a.tokens_per_group - 1u) / a.tokens_per_group : 0u));
-  const auto go = [&](auto v, auto n) {
-    constexpr int VEC = decltype(v)::value;
-    hipLaunchKernelGGL((block_append_kernel<X, KV, VEC, decltype(n)::value>), grid, dim3(threads), lds, s, a);
+  // Workgroups for each group of tokens, keys or values: as many as have tasks
+  // when its tokens are blocks of their own, or one block; 8192 in all.
+  const uint32_t longest = std::min(block, a.T), tokens = std::min(a.kv_tokens, a.T);
+  const auto parts_of = [&](uint32_t blocks, uint32_t n) {
+    uint32_t lanes = 1u;
+    while (lanes < kThreads && (lanes * kHeld<VEC> < n * row || lanes < row)) lanes *= 2u;
+    return ((uint64_t)blocks * a.heads * lanes + kThreads - 1u) / kThreads;
   };
-  using std::integral_constant;
+  const uint64_t parts = std::max(parts_of(tokens, 1u), parts_of(1u, longest));
+  a.kv_parts = (uint32_t)std::min<uint64_t>(parts, std::max(1024u / (2u * a.kv_groups), 1u));
+  // All tokens of a step of one block, and some of its neighbours'.
+  a.turn_tokens = std::min(longest, kThreads * kHeld<VEC> / row + 2u) + 15u;
+  const uint32_t lds = half * std::max(a.tokens_per_group, a.turn_tokens) * (uint32_t)sizeof(float2);
+  const uint32_t kv = a.kv_groups * 2u * a.kv_parts;
+  const dim3 grid(kv + (units ? (a.T + a.tokens_per_group - 1u) / a.tokens_per_group : 0u));
+  hipLaunchKernelGGL((block_append_kernel<X, KV, VEC, NEIGHBOURS>), grid, dim3(kThreads), lds, s, a);
+  return hipGetLastError();
+}
+
+template <class X, class KV>
+hipError_t launch(const BlockAppendArgs& a, bool neighbours, uint32_t vec, hipStream_t s) {
   // 16 bytes an access: a vector, or two neighbouring ones.
   constexpr int kWide = 16 / sizeof(typename X::Raw);
-  if (neighbours) {
-    if (vec == kWide / 2) go(integral_constant<int, kWide / 2>{}, std::true_type{});
-    else go(integral_constant<int, 1>{}, std::true_type{});
-  } else if (vec == kWide) {
-    go(integral_constant<int, kWide>{}, std::false_type{});
-  } else if (vec == kWide / 2) {
-    go(integral_constant<int, kWide / 2>{}, std::false_type{});
-  } else {
-    go(integral_constant<int, 1>{}, std::false_type{});
-  }
-  return hipGetLastError();
+  if (neighbours) return vec == kWide / 2 ? launch_vec<X, KV, kWide / 2, true>(a, s) : launch_vec<X, KV, 1, true>(a, s);
+  if (vec == kWide) return launch_vec<X, KV, kWide, false>(a, s);
+  return vec == kWide / 2 ? launch_vec<X, KV, kWide / 2, false>(a, s) : launch_vec<X, KV, 1, false>(a, s);
 }
 
 }  // namespace

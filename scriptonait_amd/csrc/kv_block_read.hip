@@ -1,8 +1,10 @@
 // Tokens' keys and values out of a cache of codes (llmhip_kv_block_read).
 //
-// A thread takes 8 codes of one head row, key or value: one load of 8 bytes,
-// one scale that the row's other threads read too, 16 or 32 bytes out. What
-// bounds it is the traffic.
+// A unit is 8 codes of one head row, key or value: one load of 8 bytes, one
+// scale that the row's other lanes read too, 16 or 32 bytes out, past the L2. A
+// thread has up to 4 units' loads on their way. What bounds it is the traffic.
+#include <algorithm>
+
 #include "kv_args.h"
 #include "kv_types.h"
 
@@ -10,47 +12,70 @@ namespace llmhip {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kMaxTokens = 32;
+constexpr uint32_t kMaxTokens = 64;
 
-template <class X, class KV>
+template <class X>
+__device__ __forceinline__ void store_once(typename X::Raw* p, const Pack<X, 8>& x) {
+  using W = uint32_t __attribute__((ext_vector_type(4)));
+  typedef W __attribute__((aligned(2))) Placed;  // rows of any alignment
+  W w[sizeof x / 16];
+  __builtin_memcpy(w, &x, sizeof x);
+#pragma unroll
+  for (uint32_t i = 0; i < sizeof x / 16; ++i) __builtin_nontemporal_store(w[i], reinterpret_cast<Placed*>(p) + i);
+}
+
+template <class X, class KV, uint32_t UNITS>
 __global__ __launch_bounds__(kThreads) void block_read_kernel(BlockReadArgs a) {
   __shared__ uint32_t s_page[kMaxTokens], s_token[kMaxTokens];
   const uint32_t tid = threadIdx.x, t0 = blockIdx.x * a.tokens_per_group, n = min(a.tokens_per_group, a.T - t0);
   if (tid < n) {
     uint32_t p = 0, t = 0;
     bool bad = false;
-    const bool live = split_slot(a.slots[t0 + tid], a.pages, a.page, p, t, bad);
+    const int64_t slot = a.slots[t0 + tid];
+    const bool live = a.short_slots ? split_short_slot(slot, a.pages, a.by_page, p, t, bad) : split_slot(slot, a.pages, a.page, p, t, bad);
     if (bad) atomicOr(a.status, LLMHIP_KSTATUS_BAD_INDEX);
     s_page[tid] = live ? p : 0xffffffffu;
     s_token[tid] = t;
   }
   __syncthreads();
-  for (uint32_t u = tid; u < n * a.by_token.d; u += kThreads) {
-    const uint32_t t = a.by_token.div(u), in_token = u - t * a.by_token.d, page = s_page[t], token = s_token[t];
-    uint32_t head = a.by_row.div(in_token);
-    const uint32_t d = (in_token - head * a.by_row.d) * 8u;
-    const uint32_t kind = head >= a.heads || !a.out[0] ? 1u : 0u;
-    head -= head >= a.heads ? a.heads : 0u;
-    Pack<KV, 8> in{};
-    float scale = 0.0f;
-    if (page != 0xffffffffu) {
-      in = *reinterpret_cast<const Pack<KV, 8>*>(static_cast<const typename KV::Raw*>(a.pool[kind]) +
-                                                 (int64_t)page * a.pool_stride[kind][0] +
-                                                 (int64_t)token * a.pool_stride[kind][1] +
-                                                 (int64_t)head * a.pool_stride[kind][2] + d);
-      scale = a.block_scales.scale[kind][(int64_t)page * a.block_scales.stride[kind][0] +
-                                   (int64_t)a.block_scales.by_block.div(token) * a.block_scales.stride[kind][1] +
-                                   (int64_t)head * a.block_scales.stride[kind][2]];
-    }
-    Pack<X, 8> x;
+  for (uint32_t u0 = tid; u0 < n * a.by_token.d; u0 += UNITS * kThreads) {
+    Pack<KV, 8> in[UNITS];
+    float scale[UNITS];
+    typename X::Raw* to[UNITS];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float y = KV::load(in.v[j]) * scale;
-      asm("" : "+v"(y));  // the product in binary32 for every type (else one instruction rounds it to float16)
-      x.v[j] = X::store(y);
+    for (uint32_t k = 0; k < UNITS; ++k) {
+      const uint32_t u = min(u0 + k * kThreads, n * a.by_token.d - 1u);
+      const uint32_t t = a.by_token.div(u), in_token = u - t * a.by_token.d, page = s_page[t], token = s_token[t];
+      uint32_t head = a.by_row.div(in_token);
+      const uint32_t d = (in_token - head * a.by_row.d) * 8u;
+      const uint32_t kind = head >= a.heads || !a.out[0] ? 1u : 0u;
+      head -= head >= a.heads ? a.heads : 0u;
+      in[k] = Pack<KV, 8>{};
+      scale[k] = 0.0f;
+      if (page != 0xffffffffu) {
+        in[k] = *reinterpret_cast<const Pack<KV, 8>*>(static_cast<const typename KV::Raw*>(a.pool[kind]) +
+                                                      (int64_t)page * a.pool_stride[kind][0] +
+                                                      (int64_t)token * a.pool_stride[kind][1] +
+                                                      (int64_t)head * a.pool_stride[kind][2] + d);
+        scale[k] = a.block_scales.scale[kind][(int64_t)page * a.block_scales.stride[kind][0] +
+                                              (int64_t)a.block_scales.by_block.div(token) * a.block_scales.stride[kind][1] +
+                                              (int64_t)head * a.block_scales.stride[kind][2]];
+      }
+      to[k] = static_cast<typename X::Raw*>(a.out[kind]) + (int64_t)(t0 + t) * a.out_stride[kind][0] +
+              (int64_t)head * a.out_stride[kind][1] + d;
     }
-    __builtin_memcpy(static_cast<typename X::Raw*>(a.out[kind]) + (int64_t)(t0 + t) * a.out_stride[kind][0] +
-                         (int64_t)head * a.out_stride[kind][1] + d, &x, sizeof x);
+#pragma unroll
+    for (uint32_t k = 0; k < UNITS; ++k) {
+      if (k && u0 + k * kThreads >= n * a.by_token.d) continue;
+      Pack<X, 8> x;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float y = KV::load(in[k].v[j]) * scale[k];
+        asm("" : "+v"(y));  // the product in binary32 for every type (else one instruction rounds it to float16)
+        x.v[j] = X::store(y);
+      }
+      store_once<X>(to[k], x);
+    }
   }
 }
 
@@ -59,8 +84,14 @@ hipError_t launch(BlockReadArgs a, hipStream_t s) {
   const uint32_t row = a.dim / 8u, units = row * a.heads * ((a.out[0] != nullptr) + (a.out[1] != nullptr));
   a.by_row = FastDiv::of(row);
   a.by_token = FastDiv::of(units);
-  a.tokens_per_group = min(max(kThreads / units, 1u), kMaxTokens);
-  hipLaunchKernelGGL((block_read_kernel<X, KV>), dim3((a.T + a.tokens_per_group - 1u) / a.tokens_per_group), dim3(kThreads), 0, s, a);
+  a.by_page = FastDiv::of(a.page);
+  a.short_slots = (uint64_t)a.pages * a.page <= 0x7fffffffu;
+  // One unit a thread where few workgroups are, else four.
+  const bool many = (uint64_t)a.T * units >= 4096u * kThreads;
+  a.tokens_per_group = std::min(std::max((many ? 4u : 1u) * kThreads / units, 1u), kMaxTokens);
+  const dim3 grid((a.T + a.tokens_per_group - 1u) / a.tokens_per_group);
+  if (many) hipLaunchKernelGGL((block_read_kernel<X, KV, 4>), grid, dim3(kThreads), 0, s, a);
+  else hipLaunchKernelGGL((block_read_kernel<X, KV, 1>), grid, dim3(kThreads), 0, s, a);
   return hipGetLastError();
 }
 

@@ -49,6 +49,18 @@ LLMHIP_HD bool split_slot(int64_t slot, uint32_t pages, uint32_t page, uint32_t&
   return true;
 }
 
+// The same of a pool below 2^31 tokens, without 64-bit divisions.
+LLMHIP_HD bool split_short_slot(int64_t slot, uint32_t pages, FastDiv page, uint32_t& p, uint32_t& t, bool& bad) {
+  if (slot < 0) return false;
+  if ((uint64_t)slot >= (uint64_t)pages * page.d) {
+    bad = true;
+    return false;
+  }
+  p = page.div((uint32_t)slot);
+  t = (uint32_t)slot - p * page.d;
+  return true;
+}
+
 // First token that a request's newest token sees.
 LLMHIP_HD uint32_t window_start(uint32_t len, uint32_t window) { return window && len > window ? len - window : 0u; }
 

@@ -95,9 +95,6 @@ def test_append_refusals():
     _refused(_append(c, out=(63, 64)), BAD, "out_q overlap")
     _refused(_append(c, out=(64, 64)), BAD, "out_q overlap")
     _refused(_append(c, T=(1 << 23) + 1), UNSUPPORTED, "T")
-    _refused(_append(_cache(heads=60000, k_stride=_three(1 << 40, 1 << 30, 64), v_stride=_three(1 << 40, 1 << 30, 64),
-                            k_scale_stride=_three(1 << 30, 1 << 20, 1), v_scale_stride=_three(1 << 30, 1 << 20, 1)),
-                     T=1 << 23, q=None, out_q=None, heads=0), UNSUPPORTED, "T times heads")
     _refused(_append(_cache(k_stride=_three(0, 512, 64))), BAD, "pool overlap")
     _refused(_append(_cache(v_stride=_three(4096, 512, 64))), BAD, "pool overlap")  # pages over one another
     _refused(_append(_cache(k_scale_stride=_three(8, 8, 1))), BAD, "scales overlap")
