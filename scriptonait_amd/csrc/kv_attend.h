@@ -121,19 +121,32 @@ struct Cut {
   uint32_t request, first, last, unused;
 };
 
-// The scales of a lane's group of tokens, of a cache that has one for each
-// block of tokens and head: N of keys and N of values, and where the cache
-// head's begin.
-template <int N>
+// The scales of a group of 8 tokens, of a cache that has one for each block of
+// tokens and head, are spread over the group's 16 lanes: lane c < 8 loads that of
+// token c's keys, lane 8 + c of its values, and a row broadcast gives all lanes
+// what they multiply with. (A load for each token and lane: 64 requests with 4 new
+// tokens and a scale for each token 75 us.)
 struct GroupScales {
-  float k[N], v[N], now[N];  // (now: of the tile at hand, times that of all scores)
-  const float* base[2];
+  float next, now;     // of the tile whose keys are loaded, and of the one at hand
+  const float* base;   // the cache head's, of the lane's kind
+  int64_t stride[2];   // page, block
 };
 struct NoScales {};
-template <class E>
-constexpr int scales_of() {
-  if constexpr (E::kBlocks) return E::kEach ? E::kGroup : 1;
-  else return 0;
+// Lane N's value of each row of 16 lanes.
+template <int N>
+__device__ __forceinline__ float row_lane(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + N, 0xf, 0xf, true));
+}
+template <int FIRST>
+__device__ __forceinline__ void row_lanes(float x, float* y) {
+  y[0] = row_lane<FIRST>(x);
+  y[1] = row_lane<FIRST + 1>(x);
+  y[2] = row_lane<FIRST + 2>(x);
+  y[3] = row_lane<FIRST + 3>(x);
+  y[4] = row_lane<FIRST + 4>(x);
+  y[5] = row_lane<FIRST + 5>(x);
+  y[6] = row_lane<FIRST + 6>(x);
+  y[7] = row_lane<FIRST + 7>(x);
 }
 
 // Query `qhead` of all of a request's (their number counts a cache head's
@@ -164,7 +177,6 @@ template <class E, bool GROUPED, bool ONCE>
 struct Run {
   static constexpr int kIds = GROUPED ? 1 : E::kGroup;       // page ids of the lane's V tokens
   static constexpr int kKIds = GROUPED ? 1 : E::kProducts;   // and of its K tokens
-  static constexpr int kScales = scales_of<E>();
   const typename E::Args& a;
   const int32_t* row;   // the request's table
   const char* base[2];  // the pools at the cache head
@@ -175,11 +187,15 @@ struct Run {
   bool far = false;  // some |m| is 2^20 or more
   bool bad = false;
   enum { kAllValues, kFinite, kInfinite } values = kAllValues;  // which ones a pass adds
-  struct Ids {
+  struct PlainIds {
     uint32_t k[kKIds], v[kIds];
   };
+  struct ScaledIds : PlainIds {
+    uint32_t scale;  // of the token whose scale the lane loads
+  };
+  using Ids = std::conditional_t<E::kBlocks && !GROUPED, ScaledIds, PlainIds>;
 
-  std::conditional_t<E::kBlocks, GroupScales<kScales ? kScales : 1>, NoScales> scales;
+  std::conditional_t<E::kBlocks, GroupScales, NoScales> scales;
   int lane_lo, lane_hi;  // kBlocks: the tokens that the lane's query sees
 
   __device__ __forceinline__ Run(const typename E::Args& args) : a(args) {}
@@ -201,6 +217,7 @@ struct Run {
     for (int p = 0; p < kKIds; ++p) x.k[p] = page_id(k_token(t0, p));
 #pragma unroll
     for (int i = 0; i < kIds; ++i) x.v[i] = page_id(v_token(t0) + i);
+    if constexpr (E::kBlocks && !GROUPED) x.scale = page_id(v_token(t0) + (c & 7u));
     return x;
   }
 
@@ -229,16 +246,18 @@ struct Run {
       for (int i = 0; i < E::kGroup; ++i) e.template load_v<ONCE>(i, token_row(1, x.v[i], a.by_page.mod(t + i)), c, a.dim);
     }
   }
-  // A scale of each of the lane's tokens, or one for all of them.
-  __device__ __forceinline__ void load_scales(float* x, int pool, uint32_t t0, const Ids& ids) const {
+  __device__ __forceinline__ void load_scales(uint32_t t0, const Ids& ids) {
     if constexpr (E::kBlocks) {
-      const uint32_t in_page = a.by_page.mod(v_token(t0));
-#pragma unroll
-      for (int i = 0; i < kScales; ++i) {
-        const uint32_t id = ids.v[GROUPED ? 0 : i], t = GROUPED ? in_page + i : a.by_page.mod(v_token(t0) + i);
-        x[i] = scales.base[pool][(int64_t)(id < a.pages ? id : 0u) * a.block_scales.stride[pool][0] +
-                                 (int64_t)a.block_scales.by_block.div(t) * a.block_scales.stride[pool][1]];
+      uint32_t id, t;
+      if constexpr (GROUPED) {
+        id = ids.v[0];
+        t = a.by_page.mod(v_token(t0)) + (E::kEach ? c & 7u : 0u);
+      } else {
+        id = ids.scale;
+        t = a.by_page.mod(v_token(t0) + (c & 7u));
       }
+      scales.next = scales.base[(int64_t)(id < a.pages ? id : 0u) * scales.stride[0] +
+                                (int64_t)a.block_scales.by_block.div(t) * scales.stride[1]];
     }
   }
   // Which of the lane's tokens are seen, as bits; kAll in every lane of most
@@ -285,9 +304,8 @@ struct Run {
     const Ids now = fetch_ids(t0);
     Ids next = fetch_ids(min(t0 + E::kTile, t_last));
     load_keys(t0, now);
-    if constexpr (E::kBlocks) load_scales(scales.k, 0, t0, now);
+    load_scales(t0, now);
     load_values(t0, now);
-    if constexpr (E::kBlocks) load_scales(scales.v, 1, t0, now);
     uint32_t seen = seen_of(t0, now);
     bool more;
     do {
@@ -298,13 +316,11 @@ struct Run {
       const Ids after = fetch_ids(min(t0 + 2u * E::kTile, t_last));
       load_keys(t1, next);
       if constexpr (E::kBlocks) {
-#pragma unroll
-        for (int i = 0; i < kScales; ++i) scales.now[i] = scales.k[i] * scale;
-        load_scales(scales.k, 0, t1, next);
+        scales.now = scales.next;
+        load_scales(t1, next);
       }
       add(s, seen);
       load_values(t1, next);
-      if constexpr (E::kBlocks) load_scales(scales.v, 1, t1, next);
       seen = seen_of(t1, next);
       next = after;
       t0 = t1;
@@ -325,15 +341,29 @@ struct Run {
     return false;
   }
 
-  // What token i's score is multiplied with.
-  static constexpr int kStep = kScales > 1 ? 1 : 0;
-  __device__ __forceinline__ float scale_of(int i) const {
-    if constexpr (E::kBlocks) return scales.now[i * kStep];
-    else return scale;
-  }
-
   // A tile's scores and values into ref, sum and o.
   __device__ __forceinline__ void add(float* s, uint32_t seen) {
+    // What each token's score is multiplied with, and its numerator.
+    float k_scale[E::kGroup], v_scale[E::kGroup];
+    if constexpr (E::kBlocks) {
+      if constexpr (E::kEach) {
+        row_lanes<0>(scales.now, k_scale);
+        row_lanes<8>(scales.now, v_scale);
+#pragma unroll
+        for (int i = 0; i < E::kGroup; ++i) k_scale[i] *= scale;
+      } else {
+        const float x = row_lane<0>(scales.now) * scale, y = row_lane<8>(scales.now);
+#pragma unroll
+        for (int i = 0; i < E::kGroup; ++i) {
+          k_scale[i] = x;
+          v_scale[i] = y;
+        }
+      }
+    }
+    const auto scale_of = [&](int i) {
+      if constexpr (E::kBlocks) return k_scale[i];
+      else return scale;
+    };
     const bool edge = __any(seen != kAll) || (E::kInfinities && values != kAllValues);
     float top = -INFINITY;
 #pragma unroll
@@ -369,13 +399,10 @@ struct Run {
           // (Whole numbers are finite whatever a place holds.)
           const bool any = seen >> (E::kGroup + i) & 1u;
           if constexpr (!std::is_same_v<typename E::KV, I8>) e.keep_v(i, any);
-          if (E::kEach) scales.v[i * kStep] = any ? scales.v[i * kStep] : 0.0f;
+          v_scale[i] = any ? v_scale[i] : 0.0f;  // (of a block that no call has written it may be no number)
         } else {
           e.keep_v(i, keep);
         }
-      }
-      if constexpr (E::kBlocks) {
-        if (!E::kEach) scales.v[0] = seen >> E::kGroup ? scales.v[0] : 0.0f;
       }
       if constexpr (E::kInfinities) {
         if (__builtin_expect(values != kAllValues, 0)) {
@@ -392,7 +419,7 @@ struct Run {
     for (int i = 0; i < E::kGroup; ++i) sum += s[i];
     if constexpr (E::kBlocks) {
 #pragma unroll
-      for (int i = 0; i < E::kGroup; ++i) s[i] *= scales.v[i * kStep];
+      for (int i = 0; i < E::kGroup; ++i) s[i] *= v_scale[i];
     }
     e.accumulate(s);
   }
@@ -473,8 +500,11 @@ __device__ __forceinline__ void attend(typename E::Args a) {
   run.scale = a.score_scale * kLog2e * (e4m3 ? a.scale[0][head] : 1.0f);
   const float vscale = e4m3 ? a.scale[1][head] : 1.0f;
   if constexpr (E::kBlocks) {
+    const int kind = run.c >= 8u;
+    run.scales.base = (kind ? a.block_scales.scale[1] : a.block_scales.scale[0]) +
+                      (int64_t)head * (kind ? a.block_scales.stride[1][2] : a.block_scales.stride[0][2]);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) run.scales.base[i] = a.block_scales.scale[i] + (int64_t)head * a.block_scales.stride[i][2];
+    for (int i = 0; i < 2; ++i) run.scales.stride[i] = kind ? a.block_scales.stride[1][i] : a.block_scales.stride[0][i];
   }
   const uint32_t qhead = head * a.group + q0;  // the first of the output
   const auto out_of = [&](uint32_t r, uint32_t qi) {
