@@ -278,6 +278,14 @@ struct Engine16 {
     else return x;
   }
 
+  // Value j of token i's in panel p, of whole numbers.
+  __device__ __forceinline__ float whole(int i, int p, int j) const {
+    uint32_t x;
+    if constexpr (kVec <= 4) x = v[i][p];
+    else x = v[i][p][j >> 2];
+    return (float)(int8_t)(x >> 8 * (j & 3));
+  }
+
   __device__ __forceinline__ static void add_product(u32x4 hi, u32x4 lo, u32x4 v, f32x4& x) {
     if constexpr (kNarrow) {
       const f32x4 y = mfma(W(), lo, v, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
@@ -315,9 +323,14 @@ struct Engine16 {
         u32x4 even, odd;  // values 2 w and 2 w + 1 of the eight tokens
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t x = word(2 * i, p, w), y = word(2 * i + 1, p, w);
-          even[i] = __builtin_amdgcn_perm(y, x, 0x05040100u);
-          odd[i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+          if constexpr (std::is_same_v<KV, I8>) {  // (two tokens' values are rounded into one word: nothing to sort after that)
+            even[i] = pack2(W(), whole(2 * i, p, 2 * w), whole(2 * i + 1, p, 2 * w));
+            odd[i] = pack2(W(), whole(2 * i, p, 2 * w + 1), whole(2 * i + 1, p, 2 * w + 1));
+          } else {
+            const uint32_t x = word(2 * i, p, w), y = word(2 * i + 1, p, w);
+            even[i] = __builtin_amdgcn_perm(y, x, 0x05040100u);
+            odd[i] = __builtin_amdgcn_perm(y, x, 0x07060302u);
+          }
         }
         add_product(hi, lo, even, o[p][2 * w]);
         add_product(hi, lo, odd, o[p][2 * w + 1]);
