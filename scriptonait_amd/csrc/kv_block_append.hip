@@ -26,6 +26,8 @@ constexpr uint32_t kMaxTokens = 8;  // of a workgroup of queries
 constexpr uint32_t kMaxGroup = 64;  // of one of keys or values: a lane's each
 
 // Units of a lane in registers: 32 values, 16 where they take more addresses.
+// (16 for all, in five waves of a SIMD and not four: 16384 tokens with 32 heads of
+// queries 81 us and 85, without queries 45 and 36, 2047 in blocks of 64 24 and 18.)
 template <int VEC>
 constexpr uint32_t kHeld = VEC >= 4 ? 16 / VEC : 8 / VEC;
 
@@ -175,18 +177,21 @@ __device__ __forceinline__ void fill_turns(float2* turns, const BlockAppendArgs&
   const uint32_t stride = a.by_half.div(kThreads);
   if (first >= min(stride, n)) return;
   const double freq = a.freqs[pair];
-  const bool many = first + stride < n;
-  const Turn step = many ? turn_of<true>((double)stride * freq) : Turn{1.0, 0.0};
-  Turn now = {1.0, 0.0};
-  int32_t at = a.positions[t0 + first], next = at;
-  int64_t expected = (int64_t)at + 1;  // of the first: no turn before it
+  Turn step = {1.0, 0.0}, now = {1.0, 0.0};
+  int32_t before = 0;
+  // (The first round is the step's own, so that the series are here once.)
 #pragma unroll 1
-  for (uint32_t i = first; i < n; i += stride, at = next) {
-    if (i + stride < n) next = a.positions[t0 + i + stride];
-    if (at == expected) now = Turn{now.cos * step.cos - now.sin * step.sin, now.cos * step.sin + now.sin * step.cos};
-    else now = turn_of<true>((double)at * freq);
-    expected = (int64_t)at + stride;
-    turns[i * half + pair] = {(float)now.cos, (float)now.sin};
+  for (uint32_t i = first + stride < n ? first - stride : first; (int32_t)i < (int32_t)n; i += stride) {
+    const bool own = (int32_t)i < 0;
+    const int32_t at = own ? (int32_t)stride : a.positions[t0 + i];
+    if (!own && i != first && (uint32_t)at - (uint32_t)before == stride) {
+      now = Turn{now.cos * step.cos - now.sin * step.sin, now.cos * step.sin + now.sin * step.cos};
+    } else {
+      now = turn_of<true>((double)at * freq);
+    }
+    if (own) step = now;
+    else turns[i * half + pair] = {(float)now.cos, (float)now.sin};
+    before = at;
   }
 }
 
@@ -263,17 +268,21 @@ __device__ __forceinline__ void write_blocks(const BlockAppendArgs& a, float2* t
     const uint32_t task = task0 + (tid >> log_lanes), me = tid & (lanes - 1u);
     const bool live = task < stop;
     const uint32_t mine = min(task, stop - 1u), r = run_of(mine), head = mine - r * a.heads;
-    const Run run = s_run[r];
-    const uint32_t units = live ? run.n * row : 0u;
+    const uint32_t units = live ? s_run[r].n * row : 0u, place = a.block_scales.by_block.mod(s_run[r].token);
 
-    const uint32_t block = a.block_scales.by_block.div(run.token), place = run.token - block * block_size;
-    const typename X::Raw* in = static_cast<const typename X::Raw*>(a.x[1 + kind]) + (int64_t)run.t0 * a.x_stride[1 + kind][0] +
-                                (int64_t)head * a.x_stride[1 + kind][1];
-    typename KV::Raw* out = static_cast<typename KV::Raw*>(a.pool[kind]) + (int64_t)run.page * a.pool_stride[kind][0] +
-                            (int64_t)run.token * a.pool_stride[kind][1] + (int64_t)head * a.pool_stride[kind][2];
-    float* scale = a.block_scales.scale[kind] + (int64_t)run.page * a.block_scales.stride[kind][0] +
-                   (int64_t)block * a.block_scales.stride[kind][1] + (int64_t)head * a.block_scales.stride[kind][2];
-    const float old = live && place ? *scale : 0.0f;
+    // (Again where they are needed: registers are what limits the workgroups of a compute unit.)
+    const auto row_out = [&] {
+      const Run to = s_run[r];
+      return static_cast<typename KV::Raw*>(a.pool[kind]) + (int64_t)to.page * a.pool_stride[kind][0] +
+             (int64_t)to.token * a.pool_stride[kind][1] + (int64_t)head * a.pool_stride[kind][2];
+    };
+    const auto scale_at = [&] {
+      const Run to = s_run[r];
+      return a.block_scales.scale[kind] + (int64_t)to.page * a.block_scales.stride[kind][0] +
+             (int64_t)a.block_scales.by_block.div(to.token) * a.block_scales.stride[kind][1] +
+             (int64_t)head * a.block_scales.stride[kind][2];
+    };
+    const float old = live && place ? *scale_at() : 0.0f;
 
     // The task's units in steps of as many as its lanes hold: read and looked at,
     // then written; of more than one step all are read again.
@@ -286,6 +295,9 @@ __device__ __forceinline__ void write_blocks(const BlockAppendArgs& a, float2* t
       const uint32_t first_unit = (writes ? p - steps : p) * step + me;
       if (!writes || steps > 1u) {
         Pack<X, 2 * VEC> raw[kHold];
+        const uint32_t t0 = s_run[r].t0;
+        const typename X::Raw* in = static_cast<const typename X::Raw*>(a.x[1 + kind]) + (int64_t)t0 * a.x_stride[1 + kind][0] +
+                                    (int64_t)head * a.x_stride[1 + kind][1];
 #pragma unroll
         for (uint32_t k = 0; k < kHold; ++k) {
           const uint32_t u = first_unit + k * lanes, i = a.by_row.div(u);
@@ -313,7 +325,7 @@ __device__ __forceinline__ void write_blocks(const BlockAppendArgs& a, float2* t
 #pragma unroll
         for (uint32_t k = 0; k < kHold; ++k) {
           const uint32_t u = first_unit + k * lanes, i = a.by_row.div(u), c = u - i * row;
-          rotate<X, VEC, NEIGHBOURS>(x[k], raw[k], u < units && c * 2u * VEC < dims, c, turns + (run.t0 + i - turned_from) * half);
+          rotate<X, VEC, NEIGHBOURS>(x[k], raw[k], u < units && c * 2u * VEC < dims, c, turns + (t0 + i - turned_from) * half);
           range_of<2 * VEC>(top, low, x[k]);
         }
       }
@@ -329,11 +341,11 @@ __device__ __forceinline__ void write_blocks(const BlockAppendArgs& a, float2* t
         s = s < 0x1p-126f ? 0.0f : s;
         s = old > s ? old : s;
         by = s > 0.0f ? 1.0f / s : 1.0f;  // (1: all finite values are so small that they round to 0)
-        if (live && me == 0u && !(place && s == old)) *scale = s;
+        if (live && me == 0u && !(place && s == old)) *scale_at() = s;
         if (live && place && s > old) {  // kept tokens: 8 codes at a time
           const float f = old / s;
           const uint32_t eights = a.dim / 8u;
-          typename KV::Raw* kept = out - (int64_t)place * a.pool_stride[kind][1];
+          typename KV::Raw* kept = row_out() - (int64_t)place * a.pool_stride[kind][1];
           for (uint32_t u = me; u < place * eights; u += lanes) {
             const uint32_t i = u / eights;
             typename KV::Raw* c = kept + (int64_t)i * a.pool_stride[kind][1] + (u - i * eights) * 8u;
@@ -346,6 +358,7 @@ __device__ __forceinline__ void write_blocks(const BlockAppendArgs& a, float2* t
       }
       if (writes) {
         const bool odd = __any(low < 0x01000000u);
+        typename KV::Raw* out = row_out();
 #pragma unroll
         for (uint32_t k = 0; k < kHold; ++k) {
           const uint32_t u = first_unit + k * lanes, i = a.by_row.div(u);
@@ -407,6 +420,7 @@ __global__ __launch_bounds__(kThreads, 4) void block_append_kernel(BlockAppendAr
 
 template <class X, class KV, int VEC, bool NEIGHBOURS>
 hipError_t launch_vec(BlockAppendArgs a, hipStream_t s) {
+  constexpr uint32_t kHold = kHeld<VEC>;
   const uint32_t row = a.dim / (2u * VEC), units = row * a.q_heads, half = a.dims / 2u, block = a.block_scales.by_block.d;
   a.by_row = FastDiv::of(row);
   a.by_token = FastDiv::of(units ? units : 1u);
@@ -423,13 +437,13 @@ hipError_t launch_vec(BlockAppendArgs a, hipStream_t s) {
   const uint32_t longest = std::min(block, a.T), tokens = std::min(a.kv_tokens, a.T);
   const auto parts_of = [&](uint32_t blocks, uint32_t n) {
     uint32_t lanes = 1u;
-    while (lanes < kThreads && (lanes * kHeld<VEC> < n * row || lanes < row)) lanes *= 2u;
+    while (lanes < kThreads && (lanes * kHold < n * row || lanes < row)) lanes *= 2u;
     return ((uint64_t)blocks * a.heads * lanes + kThreads - 1u) / kThreads;
   };
   const uint64_t parts = std::max(parts_of(tokens, 1u), parts_of(1u, longest));
   a.kv_parts = (uint32_t)std::min<uint64_t>(parts, std::max(1024u / (2u * a.kv_groups), 1u));
   // All tokens of a step of one block, and some of its neighbours'.
-  a.turn_tokens = std::min(longest, kThreads * kHeld<VEC> / row + 2u) + 15u;
+  a.turn_tokens = std::min(longest, kThreads * kHold / row + 2u) + 15u;
   const uint32_t lds = half * std::max(a.tokens_per_group, a.turn_tokens) * (uint32_t)sizeof(float2);
   const uint32_t kv = a.kv_groups * 2u * a.kv_parts;
   const dim3 grid(kv + (units ? (a.T + a.tokens_per_group - 1u) / a.tokens_per_group : 0u));
