@@ -34,7 +34,7 @@ namespace llmhip {
 
 // Waves of a workgroup: 8, two on each SIMD, where the registers allow it.
 template <class E, bool GROUPED>
-constexpr uint32_t kWavesOf = E::kDim > 128 || (!GROUPED && E::kDim > 64) || E::kLarge ? 4 : 8;
+constexpr uint32_t kWavesOf = E::kDim > 128 || (!GROUPED && E::kDim > 64) ? 4 : 8;
 constexpr float kLazyBits = 8.0f;
 constexpr float kLn2 = 0.693147180559945309f, kLog2e = 1.44269504088896341f;
 constexpr uint32_t kNoId = 0xffffffffu;

@@ -178,12 +178,14 @@ __device__ __forceinline__ void fill_turns(float2* turns, const BlockAppendArgs&
   if (first >= min(stride, n)) return;
   const double freq = a.freqs[pair];
   Turn step = {1.0, 0.0}, now = {1.0, 0.0};
-  int32_t before = 0;
-  // (The first round is the step's own, so that the series are here once.)
+  int32_t before = 0, next = a.positions[t0 + first];
+  // (The first round is the step's own, so that the series are here once. The
+  // next position is on its way while a turn is computed.)
 #pragma unroll 1
   for (uint32_t i = first + stride < n ? first - stride : first; (int32_t)i < (int32_t)n; i += stride) {
     const bool own = (int32_t)i < 0;
-    const int32_t at = own ? (int32_t)stride : a.positions[t0 + i];
+    const int32_t at = own ? (int32_t)stride : next;
+    if (!own) next = a.positions[t0 + min(i + stride, n - 1u)];
     if (!own && i != first && (uint32_t)at - (uint32_t)before == stride) {
       now = Turn{now.cos * step.cos - now.sin * step.sin, now.cos * step.sin + now.sin * step.cos};
     } else {

@@ -127,7 +127,6 @@ struct Engine16 {
   using KV = KV_;
   using Args = AttendArgs;
   static constexpr bool kBlocks = false;
-  static constexpr bool kLarge = false;  // more registers than two waves of a SIMD have
   static constexpr int kElem = sizeof(typename KV::Raw);
   static constexpr int kDim = DIM;
   static constexpr int kGroup = 8, kTile = 32, kProducts = 2;
@@ -346,7 +345,6 @@ struct BlockEngine : Engine16<Q_, KV_, DIM, FULL, CHUNK> {
   using Args = BlockAttendArgs;
   static constexpr bool kBlocks = true;
   static constexpr bool kEach = EACH;
-  static constexpr bool kLarge = EACH && CHUNK == 8 && DIM > 64;
 };
 
 // Queries and cache in binary32: the products are 4 deep, one token of each
@@ -357,7 +355,6 @@ struct Engine32 {
   using KV = F32;
   using Args = AttendArgs;
   static constexpr bool kBlocks = false;
-  static constexpr bool kLarge = false;
   static constexpr int kElem = 4;
   static constexpr int kDim = DIM;
   static constexpr int kGroup = 4, kTile = 16, kProducts = 1;
