@@ -2,15 +2,19 @@
 // rotated (llmhip_kv_block_append).
 //
 // A block's scale needs the largest of its new values before the first code
-// can be written. A workgroup finds the blocks that begin among 16 tokens (their
-// slots say so) and gives each block and head as many neighbouring lanes as
-// hold all of its new values in registers: 8 for a decoding request's single row
-// of 128 values, all 256 for 64 of them. The maximum goes across those lanes, and
-// codes are written. Of blocks that are larger the rows are read again, from
-// the L2. So a value comes from memory once. Cosines and sines are computed
-// once for all heads of a workgroup, into LDS. Kept tokens are read only where
-// the scale grew. Units are laid out as in the append to a cache of values: 2 *
-// VEC values of a row, VEC pairs, or values that are not rotated.
+// can be written. A workgroup finds the blocks that begin among some tokens (their
+// slots say so; as many as a block has, 16 to 64) and gives each block and head
+// as many neighbouring lanes as hold all of its new values in registers: 8 for a
+// decoding request's single row of 128 values, all 256 for 64 of them. The maximum
+// goes across those lanes, and codes are written. Of blocks that are larger the
+// rows are read again, from the L2. So a value comes from memory once. Cosines and
+// sines are computed once for all heads of a workgroup, into LDS. Kept tokens are
+// read only where the scale grew. Units are laid out as in the append to a cache
+// of values: 2 * VEC values of a row, VEC pairs, or values that are not rotated.
+//
+// What bounds it: for few tokens the chain slots, rows, maximum, codes (256
+// tokens 7.2 us); for many the traffic, 368 MB of 16384 tokens in 80 us, 4.6 TB/s,
+// of which the vector units are busy for 47.
 #include <algorithm>
 
 #include "kv_args.h"
@@ -86,9 +90,21 @@ __device__ __forceinline__ Pack<X, 2 * VEC> get(const typename X::Raw* row, cons
   }
 }
 
+// Where a token's pair i has its cosine and sine: lanes take VEC neighbouring
+// pairs each, two at a time, and what neighbouring lanes read at once is
+// neighbouring 16 bytes. (In their order: 16384 tokens 85 us and not 80, a fifth
+// of them with bank conflicts.)
+template <int VEC>
+__device__ __forceinline__ uint32_t turn_at(uint32_t i, uint32_t half) {
+  if (VEC < 4) return i;
+  const uint32_t c = i / VEC, j = i % VEC;
+  return ((j >> 1) * (half / VEC) + c) * 2u + (j & 1u);
+}
+
 // In binary32 and rotated; turn: its token's cosines and sines.
 template <class X, int VEC, bool NEIGHBOURS>
-__device__ __forceinline__ void rotate(float* x, const Pack<X, 2 * VEC>& in, bool turned, uint32_t c, const float2* turn) {
+__device__ __forceinline__ void rotate(float* x, const Pack<X, 2 * VEC>& in, bool turned, uint32_t c, const float2* turn,
+                                       uint32_t half) {
 #pragma unroll
   for (int j = 0; j < 2 * VEC; ++j) x[j] = X::load(in.v[j]);
   if (turned) {
@@ -96,7 +112,7 @@ __device__ __forceinline__ void rotate(float* x, const Pack<X, 2 * VEC>& in, boo
     for (int j = 0; j < VEC; ++j) {
       const int ia = NEIGHBOURS ? 2 * j : j, ib = NEIGHBOURS ? 2 * j + 1 : VEC + j;
       const float va = x[ia], vb = x[ib];
-      const float2 w = turn[c * VEC + j];
+      const float2 w = turn[turn_at<VEC>(c * VEC + j, half)];
       x[ia] = va * w.x - vb * w.y;
       x[ib] = va * w.y + vb * w.x;
     }
@@ -172,10 +188,12 @@ __device__ __forceinline__ float magnitude(uint32_t top) {
 // one pair; while positions go on as tokens do, the next turn is the one before
 // and a step's: four products and not two series, each of which adds no more
 // than 2^-51 (the 80 steps that LDS holds, 2^-44).
+template <int VEC>
 __device__ __forceinline__ void fill_turns(float2* turns, const BlockAppendArgs& a, uint32_t t0, uint32_t n) {
   const uint32_t half = a.by_half.d, first = a.by_half.div(threadIdx.x), pair = threadIdx.x - first * half;
   const uint32_t stride = a.by_half.div(kThreads);
   if (first >= min(stride, n)) return;
+  const uint32_t place = turn_at<VEC>(pair, half);
   const double freq = a.freqs[pair];
   Turn step = {1.0, 0.0}, now = {1.0, 0.0};
   int32_t before = 0, next = a.positions[t0 + first];
@@ -192,7 +210,7 @@ __device__ __forceinline__ void fill_turns(float2* turns, const BlockAppendArgs&
       now = turn_of<true>((double)at * freq);
     }
     if (own) step = now;
-    else turns[i * half + pair] = {(float)now.cos, (float)now.sin};
+    else turns[i * half + place] = {(float)now.cos, (float)now.sin};
     before = at;
   }
 }
@@ -318,7 +336,7 @@ __device__ __forceinline__ void write_blocks(const BlockAppendArgs& a, float2* t
           }
           if (turned_from != turns_from || to != turns_to) {
             __syncthreads();  // (the ones before are used)
-            fill_turns(turns, a, turned_from, to > turned_from ? to - turned_from : 0u);  // (a shorter run has none in the last steps)
+            fill_turns<VEC>(turns, a, turned_from, to > turned_from ? to - turned_from : 0u);  // (a shorter run has none in the last steps)
             __syncthreads();
             turns_from = turned_from;
             turns_to = to;
@@ -327,7 +345,8 @@ __device__ __forceinline__ void write_blocks(const BlockAppendArgs& a, float2* t
 #pragma unroll
         for (uint32_t k = 0; k < kHold; ++k) {
           const uint32_t u = first_unit + k * lanes, i = a.by_row.div(u), c = u - i * row;
-          rotate<X, VEC, NEIGHBOURS>(x[k], raw[k], u < units && c * 2u * VEC < dims, c, turns + (t0 + i - turned_from) * half);
+          rotate<X, VEC, NEIGHBOURS>(x[k], raw[k], u < units && c * 2u * VEC < dims, c, turns + (t0 + i - turned_from) * half,
+                                     half);
           range_of<2 * VEC>(top, low, x[k]);
         }
       }
@@ -403,7 +422,7 @@ __global__ __launch_bounds__(kThreads, 4) void block_append_kernel(BlockAppendAr
   unit_at(min(tid, units - 1u), t, head, c);
   Pack<X, 2 * VEC> in = get<X, VEC, NEIGHBOURS>(row_of(t, head), unit_of<VEC, NEIGHBOURS>(c, a.dims, a.dim));
   if (half) {
-    fill_turns(s_turn, a, t0, n);
+    fill_turns<VEC>(s_turn, a, t0, n);
     __syncthreads();
   }
 #pragma unroll 1
@@ -414,7 +433,7 @@ __global__ __launch_bounds__(kThreads, 4) void block_append_kernel(BlockAppendAr
     }
     const Unit at = unit_of<VEC, NEIGHBOURS>(c, a.dims, a.dim);
     float x[2 * VEC];
-    rotate<X, VEC, NEIGHBOURS>(x, in, at.turned, c, s_turn + t * half);
+    rotate<X, VEC, NEIGHBOURS>(x, in, at.turned, c, s_turn + t * half, half);
     put<X, VEC, NEIGHBOURS>(static_cast<typename X::Raw*>(a.out_q) + (int64_t)(t0 + t) * a.oq_stride[0] +
                                 (int64_t)head * a.oq_stride[1], at, x, 1.0f);
   }
@@ -435,7 +454,9 @@ hipError_t launch_vec(BlockAppendArgs a, hipStream_t s) {
   a.kv_tokens = std::min(std::max(block, 16u), kMaxGroup);
   a.kv_groups = (a.T + a.kv_tokens - 1u) / a.kv_tokens;
   // Workgroups for each group of tokens, keys or values: as many as have tasks
-  // when its tokens are blocks of their own, or one block; 8192 in all.
+  // when its tokens are blocks of their own, or one block; 1024 in all, as each
+  // that finds no task has read the slots for nothing (16384 tokens 90 us, with
+  // 8192 workgroups 130).
   const uint32_t longest = std::min(block, a.T), tokens = std::min(a.kv_tokens, a.T);
   const auto parts_of = [&](uint32_t blocks, uint32_t n) {
     uint32_t lanes = 1u;
