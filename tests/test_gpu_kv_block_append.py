@@ -134,6 +134,8 @@ def test_codes_and_scales_without_a_rotation(sampler, q, kv, lens, Hq, H, D, pag
     ([(9, 33)], 3, 9, 40, 36, 11, 11),
     ([(5, 20)], 6, 2, 24, 6, 4, 4),
     ([(0, 513)], 1, 1, 16, 16, 256, 128),
+    ([(5, 2500)], 2, 33, 64, 64, 32, 16),
+    ([(0, 300), (17, 270)], 1, 2, 256, 128, 256, 256),
 ])
 def test_rotated_keys_and_queries(sampler, q, kv, style, lens, Hq, H, D, dims, page, block):
     import torch
@@ -273,4 +275,47 @@ def test_rows_of_any_place_and_a_query_in_place(sampler):
     empty = torch.zeros(0, 2, 64, device="cuda")
     got, _ = run_append(sampler, pools, scales, empty, empty, np.zeros(0, np.int64))
     for a, b in zip(got, (*pools, *scales)):
+        same(a, b)
+
+
+@pytest.mark.parametrize("kv", ["i8", "e4m3"])
+def test_more_heads_and_tokens_than_workgroups(sampler, kv):
+    """Workgroups that take several heads of several blocks, one after the other."""
+    import torch
+
+    g = torch.Generator().manual_seed(9)
+    T, H, D, page, block = 3000, 41, 32, 32, 16
+    pools, scales = make_pools(g, 100, page, H, D, block, kv)
+    slots, _ = make_slots(np.random.RandomState(9), [(5, 1700), (0, 1), (40, 1296)], page, 100)
+    x = torch.randn(len(slots), 2 * H, D, generator=g).to(torch.bfloat16)
+    on = x.cuda()
+    got, _ = run_append(sampler, pools, scales, on[:, :H], on[:, H:], slots)
+    for i in range(2):
+        pool, scale = kv_block_oracle.write(pools[i], scales[i], x[:, i * H:(i + 1) * H].float(), slots.tolist())
+        same(got[2 + i], scale)
+        same(got[i], pool)
+    assert T <= len(slots)
+
+
+@pytest.mark.parametrize("H", [1, 3, 40])
+def test_a_batch_is_its_tokens_one_by_one(sampler, H):
+    """Decoding requests far apart in a padded batch, with rotations: what each
+    writes does not depend on the others."""
+    import torch
+
+    from scriptonait_amd.kv import Rope
+
+    g, rs = torch.Generator().manual_seed(H), np.random.RandomState(H)
+    T, D, page, block = 200, 256, 64, 64
+    pools, scales = make_pools(g, T, page, H, D, block, "i8")
+    slots, pos = np.full(T, -1), rs.randint(0, 1 << 20, T)
+    live = [0, 1, 30, 55, 63, 64, 100, 127, 128, 190, 199]
+    slots[live] = rs.permutation(T)[:len(live)] * page + rs.randint(0, page, len(live))
+    k, v = (torch.randn(T, H, D, generator=g).bfloat16().cuda() for _ in range(2))
+    rope = Rope(D)
+    whole, _ = run_append(sampler, pools, scales, k, v, slots, positions=pos, rope=rope)
+    state = [*pools, *scales]
+    for t in live:
+        state, _ = run_append(sampler, state[:2], state[2:], k[t:t + 1], v[t:t + 1], slots[t:t + 1], positions=pos[t:t + 1], rope=rope)
+    for a, b in zip(whole, state):
         same(a, b)
