@@ -13,7 +13,7 @@
 // of values: 2 * VEC values of a row, VEC pairs, or values that are not rotated.
 //
 // What bounds it: for few tokens the chain slots, rows, maximum, codes (256
-// tokens 7.2 us); for many the traffic, 368 MB of 16384 tokens in 80 us, 4.6 TB/s,
+// tokens 7.3 us); for many the traffic, 368 MB of 16384 tokens in 78 us, 4.7 TB/s,
 // of which the vector units are busy for 47.
 #include <algorithm>
 
@@ -27,6 +27,7 @@ namespace {
 
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kMaxTokens = 8;  // of a workgroup of queries
+constexpr uint32_t kMaxTurned = 256 + 15;  // tokens whose cosines and sines LDS holds: a block's, and some more
 constexpr uint32_t kMaxGroup = 64;  // of one of keys or values: a lane's each
 
 // Units of a lane in registers: 32 values, 16 where they take more addresses.
@@ -184,26 +185,28 @@ __device__ __forceinline__ float magnitude(uint32_t top) {
   return top < 0x01000000u ? 0.0f : __uint_as_float((top - 0x01000000u) >> 1);
 }
 
-// Cosines and sines of n tokens from t0 on. A thread takes every few tokens of
+// Cosines and sines of n tokens at these positions. A thread takes every few tokens of
 // one pair; while positions go on as tokens do, the next turn is the one before
 // and a step's: four products and not two series, each of which adds no more
 // than 2^-51 (the 80 steps that LDS holds, 2^-44).
+// (positions: in LDS where there are many. Read from memory, one ahead of the
+// loop, 16384 tokens take 80 us and not 77.5, 2047 in blocks of 64 17.8 and not 17.2.)
 template <int VEC>
-__device__ __forceinline__ void fill_turns(float2* turns, const BlockAppendArgs& a, uint32_t t0, uint32_t n) {
+__device__ __forceinline__ void fill_turns(float2* turns, const BlockAppendArgs& a, const int32_t* positions, uint32_t n) {
   const uint32_t half = a.by_half.d, first = a.by_half.div(threadIdx.x), pair = threadIdx.x - first * half;
   const uint32_t stride = a.by_half.div(kThreads);
   if (first >= min(stride, n)) return;
   const uint32_t place = turn_at<VEC>(pair, half);
   const double freq = a.freqs[pair];
   Turn step = {1.0, 0.0}, now = {1.0, 0.0};
-  int32_t before = 0, next = a.positions[t0 + first];
+  int32_t before = 0, next = positions[first];
   // (The first round is the step's own, so that the series are here once. The
   // next position is on its way while a turn is computed.)
 #pragma unroll 1
   for (uint32_t i = first + stride < n ? first - stride : first; (int32_t)i < (int32_t)n; i += stride) {
     const bool own = (int32_t)i < 0;
     const int32_t at = own ? (int32_t)stride : next;
-    if (!own) next = a.positions[t0 + min(i + stride, n - 1u)];
+    if (!own) next = positions[min(i + stride, n - 1u)];
     if (!own && i != first && (uint32_t)at - (uint32_t)before == stride) {
       now = Turn{now.cos * step.cos - now.sin * step.sin, now.cos * step.sin + now.sin * step.cos};
     } else {
@@ -228,6 +231,7 @@ __device__ __forceinline__ void write_blocks(const BlockAppendArgs& a, float2* t
   constexpr uint32_t kHold = kHeld<VEC>;
   __shared__ Run s_run[kMaxGroup];
   __shared__ uint32_t s_top[kThreads / 64];
+  __shared__ int32_t s_position[kMaxTurned];
   const uint32_t tid = threadIdx.x, lane = lane_id(), wave = readlane_u32(tid >> 6, 0);
   const uint32_t begin = group * a.kv_tokens, size = min(a.kv_tokens, a.T - begin), t = begin + lane;
 
@@ -335,8 +339,10 @@ __device__ __forceinline__ void write_blocks(const BlockAppendArgs& a, float2* t
             to = min(upto, from + a.by_row.div(unit0 + step - 1u) + 1u);
           }
           if (turned_from != turns_from || to != turns_to) {
-            __syncthreads();  // (the ones before are used)
-            fill_turns<VEC>(turns, a, turned_from, to > turned_from ? to - turned_from : 0u);  // (a shorter run has none in the last steps)
+            const uint32_t tokens = to > turned_from ? to - turned_from : 0u;  // (a shorter run has none in the last steps)
+            for (uint32_t i = tid; i < tokens; i += kThreads) s_position[i] = a.positions[turned_from + i];
+            __syncthreads();  // (and the turns before are used)
+            fill_turns<VEC>(turns, a, s_position, tokens);
             __syncthreads();
             turns_from = turned_from;
             turns_to = to;
@@ -422,7 +428,7 @@ __global__ __launch_bounds__(kThreads, 4) void block_append_kernel(BlockAppendAr
   unit_at(min(tid, units - 1u), t, head, c);
   Pack<X, 2 * VEC> in = get<X, VEC, NEIGHBOURS>(row_of(t, head), unit_of<VEC, NEIGHBOURS>(c, a.dims, a.dim));
   if (half) {
-    fill_turns<VEC>(s_turn, a, t0, n);
+    fill_turns<VEC>(s_turn, a, a.positions + t0, n);
     __syncthreads();
   }
 #pragma unroll 1
