@@ -272,7 +272,7 @@ int llmhip_kv_block_attend_workspace(llmhip_ctx* ctx, const llmhip_kv_blocks* ca
  * All else is as there. Scales of tokens that are seen have to be finite; what
  * is behind a request's length (codes and scales) is never used. Each softmax
  * weight times its value's scale is rounded to binary32 and meets the codes as
- * the sum of two bfloat16: off by at most 2^-16 of itself.
+ * the sum of two bfloat16: off by at most 2^-16 of itself, or 2^-125.
  */
 int llmhip_kv_block_attend(llmhip_ctx* ctx, const llmhip_kv_blocks* cache, uint32_t dtype, size_t B, size_t new_tokens,
                            size_t q_heads, const void* q, int64_t q_request, int64_t q_token, int64_t q_head,

@@ -458,7 +458,7 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 template <class E, bool GROUPED, bool ONCE>
 __device__ __forceinline__ void attend(typename E::Args a) {
   constexpr uint32_t kWaves = kWavesOf<E, GROUPED>;
-  extern __shared__ uint32_t s_mem[];
+  extern __shared__ __attribute__((aligned(16))) uint32_t s_mem[];
   __shared__ int32_t s_slot[2 * kWaves];  // the request of each partial answer, or -1
   float* s_part = reinterpret_cast<float*>(s_mem + a.start_words);
 
@@ -528,8 +528,17 @@ __device__ __forceinline__ void attend(typename E::Args a) {
       for (uint32_t p = 0; p < E::kPanels; ++p) {
         const uint32_t d = (p * 16u + run.c) * E::kVec;
         if (d >= a.dim) continue;
+        // (In stores of 16 bytes, or 8: the compiler joins none, and 16 queries of
+        // 64 requests, over whole numbers, take 66 us then, not 60.)
+        using Store = float __attribute__((ext_vector_type(E::kVec < 4 ? E::kVec : 4)));
+        constexpr int kEach = sizeof(Store) / 4;
 #pragma unroll
-        for (int j = 0; j < E::kVec; ++j) part[qi * a.dim + d + j] = run.e.o[p][j][i];
+        for (int j = 0; j < E::kVec; j += kEach) {
+          Store x;
+#pragma unroll
+          for (int k = 0; k < kEach; ++k) x[k] = run.e.o[p][j + k][i];
+          *reinterpret_cast<Store*>(part + qi * a.dim + d + j) = x;
+        }
       }
     }
     if (lane < group) {
