@@ -827,9 +827,18 @@ hipError_t launch_attend_engine(const typename E::Args& a, hipStream_t s) {
   if constexpr (E::kDim == 32) {
     return grouped ? launch_attend_group<E, true, false>(a, s) : launch_attend_group<E, false, false>(a, s);
   } else {
-    if (!grouped) return launch_attend_group<E, false, true>(a, s);
     const uint64_t pool = (uint64_t)a.pages * a.page * a.heads * a.dim * E::kElem;
-    return pool > (64u << 20) ? launch_attend_group<E, true, true>(a, s) : launch_attend_group<E, true, false>(a, s);
+    if constexpr (E::kBlocks) {
+      // (Nor where a cache head has more queries than the matrix cores take at once,
+      // whose waves read the same rows: 135 requests of 1656 tokens with 20 for each of
+      // 8 heads of 112 203 us, past the caches 248.)
+      const bool once = pool > (64u << 20) && a.blocks == 1u;
+      if (!grouped) return once ? launch_attend_group<E, false, true>(a, s) : launch_attend_group<E, false, false>(a, s);
+      return once ? launch_attend_group<E, true, true>(a, s) : launch_attend_group<E, true, false>(a, s);
+    } else {
+      if (!grouped) return launch_attend_group<E, false, true>(a, s);
+      return pool > (64u << 20) ? launch_attend_group<E, true, true>(a, s) : launch_attend_group<E, true, false>(a, s);
+    }
   }
 }
 
