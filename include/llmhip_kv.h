@@ -270,7 +270,8 @@ int llmhip_kv_block_attend_workspace(llmhip_ctx* ctx, const llmhip_kv_blocks* ca
  *   out_lse    device nullable [B][new_tokens][q_heads] f32
  *
  * All else is as there. Scales of tokens that are seen have to be finite; what
- * is behind a request's length (codes and scales) is never used. Each softmax
+ * is behind a request's length (codes and scales) is never used. A code that is
+ * no number makes those outputs NaN that see its token, and no others. Each softmax
  * weight times its value's scale is rounded to binary32 and meets the codes as
  * the sum of two bfloat16: off by at most 2^-16 of itself, or 2^-125.
  */

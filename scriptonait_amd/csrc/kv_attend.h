@@ -186,7 +186,7 @@ struct Run {
   float ref, limit, sum = 0.0f;  // m (0 before the first finite score), what no score passes, the lane's part of l
   bool far = false;  // some |m| is 2^20 or more
   bool bad = false;
-  enum { kAllValues, kFinite, kInfinite } values = kAllValues;  // which ones a pass adds
+  enum { kAllValues, kFinite, kInfinite, kNoNumbers } values = kAllValues;  // which ones a pass adds
   struct PlainIds {
     uint32_t k[kKIds], v[kIds];
   };
@@ -295,9 +295,9 @@ struct Run {
     if (!E::kInfinities || values != kInfinite) {
       ref = 0.0f;
       far = false;
-      limit = -INFINITY;
+      limit = E::kNaNs && values == kNoNumbers ? INFINITY : -INFINITY;  // (marks are not scaled)
       sum = 0.0f;
-      e.clear();
+      if (!E::kNaNs || values != kFinite) e.clear();
     }
     uint32_t t0 = readlane_u32(first, 0) * E::kTile;  // (the same in every lane: the loop's branch is the wave's)
     const uint32_t t_last = (readlane_u32(last, 0) - 1u) * E::kTile;
@@ -328,13 +328,23 @@ struct Run {
     if (E::kInfinities && values == kInfinite) sum = before;
   }
 
-  // Whether the tiles have to be read again, for sums that are not finite: a
-  // second pass adds the finite values alone, a third the others, which their
-  // signs decide.
+  // Whether the tiles have to be read again, for sums that are not finite. Of
+  // infinite values a second pass adds the finite values alone, a third the others,
+  // which their signs decide. Of several new tokens' queries, which do not see
+  // the same tokens, and values that are no numbers (0 times one is none) a second
+  // pass counts for each query those that it sees, and a third adds the numbers
+  // to NaN where there is one, to 0 elsewhere.
   __device__ __forceinline__ bool again() {
     if constexpr (E::kInfinities) {
       if (__builtin_expect(values != kAllValues || __any(e.infinite()), 0)) {
         values = values == kAllValues ? kFinite : values == kFinite ? kInfinite : kAllValues;
+        return values != kAllValues;
+      }
+    }
+    if constexpr (E::kNaNs) {
+      if (__builtin_expect(values != kAllValues || (a.tokens > 1u && __any(e.infinite())), 0)) {
+        if (values == kNoNumbers) e.spoil();
+        values = values == kAllValues ? kNoNumbers : values == kNoNumbers ? kFinite : kAllValues;
         return values != kAllValues;
       }
     }
@@ -364,7 +374,7 @@ struct Run {
       if constexpr (E::kBlocks) return k_scale[i];
       else return scale;
     };
-    const bool edge = __any(seen != kAll) || (E::kInfinities && values != kAllValues);
+    const bool edge = __any(seen != kAll) || ((E::kInfinities || E::kNaNs) && values != kAllValues);
     float top = -INFINITY;
 #pragma unroll
     for (int i = 0; i < E::kGroup; ++i) {
@@ -411,6 +421,17 @@ struct Run {
             // A numerator above 0 whose two parts are.
             if (values == kInfinite) s[i] = s[i] > 0.0f ? 1.0f + 0x1p-12f : s[i];
             e.keep_finite(i, values == kFinite);
+          }
+        }
+      }
+      if constexpr (E::kNaNs) {
+        if (__builtin_expect(values != kAllValues, 0)) {
+#pragma unroll
+          for (int i = 0; i < E::kGroup; ++i) {
+            const bool marks = values == kNoNumbers;
+            e.keep_numbers(i, marks);
+            s[i] = marks ? (seen >> i & 1u ? 1.0f : 0.0f) : s[i];
+            v_scale[i] = marks ? 1.0f : v_scale[i];
           }
         }
       }

@@ -147,6 +147,7 @@ struct Engine16 {
   // Infinite values need passes of their own: 0 times them is NaN, and the
   // second part of a numerator is often 0 or negative.
   static constexpr bool kInfinities = kElem == 2;
+  static constexpr bool kNaNs = false;
   using KRaw = typename RawOf<CHUNK * kElem>::type;
   using VRaw = typename RawOf<kVec * kElem>::type;
 
@@ -268,6 +269,34 @@ struct Engine16 {
       }
   }
 
+  // Of token i's values, in E4M3, only those that are numbers; or (mark) 1 in the
+  // place of each that is none and 0 for all others.
+  __device__ __forceinline__ static uint32_t numbers4(uint32_t x, bool mark) {
+    const uint32_t top = ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // of bytes whose other bits are all set
+    const uint32_t none = top | (top - (top >> 7));
+    return mark ? none & 0x38383838u : x & ~none;
+  }
+  __device__ __forceinline__ void keep_numbers(int i, bool mark) {
+#pragma unroll
+    for (int p = 0; p < kPanels; ++p) {
+      if constexpr (kVec <= 4) {
+        v[i][p] = (VRaw)numbers4(v[i][p], mark);
+      } else {
+#pragma unroll
+        for (int w = 0; w < kVec / 4; ++w) v[i][p][w] = numbers4(v[i][p][w], mark);
+      }
+    }
+  }
+  // What was marked: no number.
+  __device__ __forceinline__ void spoil() {
+#pragma unroll
+    for (int p = 0; p < kPanels; ++p)
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[p][j][r] = o[p][j][r] > 0.0f ? NAN : 0.0f;
+  }
+
   // Word w (values 2 w and 2 w + 1) of token i's values in panel p.
   __device__ __forceinline__ uint32_t word(int i, int p, int w) const {
     uint32_t x;
@@ -345,6 +374,7 @@ struct BlockEngine : Engine16<Q_, KV_, DIM, FULL, CHUNK> {
   using Args = BlockAttendArgs;
   static constexpr bool kBlocks = true;
   static constexpr bool kEach = EACH;
+  static constexpr bool kNaNs = std::is_same_v<KV_, E4M3>;
 };
 
 // Queries and cache in binary32: the products are 4 deep, one token of each
@@ -360,7 +390,7 @@ struct Engine32 {
   static constexpr int kGroup = 4, kTile = 16, kProducts = 1;
   static constexpr int kSteps = DIM / 16;
   static constexpr float kLift = 0.0f;
-  static constexpr bool kInfinities = false;
+  static constexpr bool kInfinities = false, kNaNs = false;
   static constexpr int kVec = DIM % 64 ? 2 : 4, kPanels = DIM / (16 * kVec);
   using VRaw = float __attribute__((ext_vector_type(kVec)));
 
