@@ -230,9 +230,10 @@ typedef struct llmhip_kv_blocks {
  * in binary32. A value is off by half a step: s / 2 (I8), 2^-4 of itself or
  * 2^-10 s (E4M3), and once more by as much of the new step whenever a later
  * token of its block raises the scale. A block's scale falls when its first
- * token is written again. An s_new below 2^-126 is 0, and codes of a scale of 0
- * are 0. Infinite values are not looked at for s and stored as +-MAX; NaN is
- * stored as 0 (I8) or NaN (E4M3).
+ * token is written again. An s_new below 2^-126 is 0, and finite values' codes
+ * at a scale of 0 are 0. Infinite and NaN values are not looked at for s: an
+ * infinite one is stored as +-MAX whatever s is (at a scale of 0 that stands for
+ * 0), NaN as 0 (I8) or NaN (E4M3, which no scale makes a number).
  */
 int llmhip_kv_block_append(llmhip_ctx* ctx, const llmhip_kv_blocks* cache, uint32_t dtype, size_t T, const void* k,
                            int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
