@@ -175,6 +175,7 @@ __device__ __forceinline__ int64_t out_token(const BlockAttendArgs& a) { return 
 // cache again.
 template <class E, bool GROUPED, bool ONCE>
 struct Run {
+  static_assert(GROUPED || !E::kWhole, "no call has such pages");
   static constexpr int kIds = GROUPED ? 1 : E::kGroup;       // page ids of the lane's V tokens
   static constexpr int kKIds = GROUPED ? 1 : E::kProducts;   // and of its K tokens
   const typename E::Args& a;
@@ -838,15 +839,22 @@ hipError_t launch_attend_group(typename E::Args a, hipStream_t s) {
   return hipGetLastError();
 }
 
+template <class E, bool ONCE>
+hipError_t launch_attend_pages(const typename E::Args& a, hipStream_t s) {
+  if constexpr (!E::kWhole) {
+    if (a.page % E::kGroup) return launch_attend_group<E, false, ONCE>(a, s);
+  }
+  return launch_attend_group<E, true, ONCE>(a, s);
+}
+
 // Values are read past the caches unless the next call may find them there (the
 // card keeps 256 MB: pools of up to 64 MiB each), or the heads beside them on
 // their cache lines do. 537 MB 96 us and 102 with plain loads, 2.2 GB of E4M3 346
 // and 379; 67 MB of one head 26.4 and 24.9, 205 MB of rows of 32 bytes 89 and 75.
 template <class E>
 hipError_t launch_attend_engine(const typename E::Args& a, hipStream_t s) {
-  const bool grouped = a.page % E::kGroup == 0u;
   if constexpr (E::kDim == 32) {
-    return grouped ? launch_attend_group<E, true, false>(a, s) : launch_attend_group<E, false, false>(a, s);
+    return launch_attend_pages<E, false>(a, s);
   } else {
     const uint64_t pool = (uint64_t)a.pages * a.page * a.heads * a.dim * E::kElem;
     if constexpr (E::kBlocks) {
@@ -854,10 +862,9 @@ hipError_t launch_attend_engine(const typename E::Args& a, hipStream_t s) {
       // whose waves read the same rows: 135 requests of 1656 tokens with 20 for each of
       // 8 heads of 112 203 us, past the caches 248.)
       const bool once = pool > (64u << 20) && a.blocks == 1u;
-      if (!grouped) return once ? launch_attend_group<E, false, true>(a, s) : launch_attend_group<E, false, false>(a, s);
-      return once ? launch_attend_group<E, true, true>(a, s) : launch_attend_group<E, true, false>(a, s);
+      return once ? launch_attend_pages<E, true>(a, s) : launch_attend_pages<E, false>(a, s);
     } else {
-      if (!grouped) return launch_attend_group<E, false, true>(a, s);
+      if (a.page % E::kGroup) return launch_attend_group<E, false, true>(a, s);
       return pool > (64u << 20) ? launch_attend_group<E, true, true>(a, s) : launch_attend_group<E, true, false>(a, s);
     }
   }

@@ -126,7 +126,7 @@ struct Engine16 {
   using Q = Q_;
   using KV = KV_;
   using Args = AttendArgs;
-  static constexpr bool kBlocks = false;
+  static constexpr bool kBlocks = false, kWhole = false;
   static constexpr int kElem = sizeof(typename KV::Raw);
   static constexpr int kDim = DIM;
   static constexpr int kGroup = 8, kTile = 32, kProducts = 2;
@@ -374,6 +374,7 @@ struct BlockEngine : Engine16<Q_, KV_, DIM, FULL, CHUNK> {
   using Args = BlockAttendArgs;
   static constexpr bool kBlocks = true;
   static constexpr bool kEach = EACH;
+  static constexpr bool kWhole = !EACH;  // (blocks divide pages)
   static constexpr bool kNaNs = std::is_same_v<KV_, E4M3>;
 };
 
@@ -384,7 +385,7 @@ struct Engine32 {
   using Q = F32;
   using KV = F32;
   using Args = AttendArgs;
-  static constexpr bool kBlocks = false;
+  static constexpr bool kBlocks = false, kWhole = false;
   static constexpr int kElem = 4;
   static constexpr int kDim = DIM;
   static constexpr int kGroup = 4, kTile = 16, kProducts = 1;
