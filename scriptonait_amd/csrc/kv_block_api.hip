@@ -4,6 +4,7 @@
 #include <stdint.h>
 #include <string.h>
 
+#include "kv_block_tasks.h"
 #include "kv_check.h"
 
 using namespace llmhip;
@@ -92,14 +93,8 @@ int llmhip_kv_block_append(llmhip_ctx* ctx, const llmhip_kv_blocks* cache, uint3
       "scales overlap");
   const int64_t out_q_stride[2] = {out_q_token, out_q_head};
   TRY(check_out(out_q, out_q_stride, T, q_heads, dim, "rows of out_q overlap"));
-  // The widest vectors that the pairs' places allow: of 16 bytes, or of 8, or
-  // single values; of neighbouring pairs two vectors are one access.
-  const uint32_t elem = size_of(dtype);
   const bool neighbours = rope && rope->style == LLMHIP_ROPE_NEIGHBOURS;
-  uint32_t vec = (neighbours ? 8 : 16) / elem;
-  const uint32_t least = 8 / elem;
-  while (vec >= least && (dims % (2 * vec) || (dim - dims) % (2 * vec))) vec /= 2;
-  if (vec < least) vec = 1;
+  const uint32_t vec = append_vec(size_of(dtype), neighbours, dims, dim);
   ON_DEVICE(info);
   BlockAppendArgs a{};
   a.x[0] = q;

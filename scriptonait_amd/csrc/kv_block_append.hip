@@ -18,6 +18,7 @@
 #include <algorithm>
 
 #include "kv_args.h"
+#include "kv_block_tasks.h"
 #include "kv_turn.h"
 #include "kv_types.h"
 #include "wave_ops.h"
@@ -25,16 +26,11 @@
 namespace llmhip {
 namespace {
 
-constexpr uint32_t kThreads = 256;
-constexpr uint32_t kMaxTokens = 8;  // of a workgroup of queries
-constexpr uint32_t kMaxTurned = 256 + 15;  // tokens whose cosines and sines LDS holds: a block's, and some more
+constexpr uint32_t kThreads = kAppendThreads;
 constexpr uint32_t kMaxGroup = 64;  // of one of keys or values: a lane's each
 
-// Units of a lane in registers: 32 values, 16 where they take more addresses.
-// (16 for all, in five waves of a SIMD and not four: 16384 tokens with 32 heads of
-// queries 81 us and 85, without queries 45 and 36, 2047 in blocks of 64 24 and 18.)
 template <int VEC>
-constexpr uint32_t kHeld = VEC >= 4 ? 16 / VEC : 8 / VEC;
+constexpr uint32_t kHeld = append_held(VEC);
 
 template <int BYTES>
 struct Word;
@@ -187,8 +183,9 @@ __device__ __forceinline__ float magnitude(uint32_t top) {
 
 // Cosines and sines of n tokens at these positions. A thread takes every few tokens of
 // one pair; while positions go on as tokens do, the next turn is the one before
-// and a step's: four products and not two series, each of which adds no more
-// than 2^-51 (the 80 steps that LDS holds, 2^-44).
+// and a step's: four products and not two series. The angles' roundings come to
+// 2^-53 of the table's whole turn, those of cosines, sines, products and sums to
+// 2^-50 a step, of which a table has 31 at most one after the other: 2^-45.
 // (positions: in LDS where there are many. Read from memory, one ahead of the
 // loop, 16384 tokens take 80 us and not 77.5, 2047 in blocks of 64 17.8 and not 17.2.)
 template <int VEC>
@@ -455,7 +452,7 @@ hipError_t launch_vec(BlockAppendArgs a, hipStream_t s) {
   a.by_heads = FastDiv::of(a.heads);
   a.by_page = FastDiv::of(a.page);
   a.short_slots = (uint64_t)a.pages * a.page <= 0x7fffffffu;
-  a.tokens_per_group = units ? std::min(std::max(kThreads / units, 1u), kMaxTokens) : 1u;
+  a.tokens_per_group = units ? std::min(std::max(kThreads / units, 1u), kMaxQueryTokens) : 1u;
   // About the tokens of a block, so that a workgroup seldom finds none that begins.
   a.kv_tokens = std::min(std::max(block, 16u), kMaxGroup);
   a.kv_groups = (a.T + a.kv_tokens - 1u) / a.kv_tokens;
@@ -471,8 +468,7 @@ hipError_t launch_vec(BlockAppendArgs a, hipStream_t s) {
   };
   const uint64_t parts = std::max(parts_of(tokens, 1u), parts_of(1u, longest));
   a.kv_parts = (uint32_t)std::min<uint64_t>(parts, std::max(1024u / (2u * a.kv_groups), 1u));
-  // All tokens of a step of one block, and some of its neighbours'.
-  a.turn_tokens = std::min(longest, kThreads * kHold / row + 2u) + 15u;
+  a.turn_tokens = append_turn_tokens(longest, VEC, a.dim);
   const uint32_t lds = half * std::max(a.tokens_per_group, a.turn_tokens) * (uint32_t)sizeof(float2);
   const uint32_t kv = a.kv_groups * 2u * a.kv_parts;
   const dim3 grid(kv + (units ? (a.T + a.tokens_per_group - 1u) / a.tokens_per_group : 0u));
