@@ -251,7 +251,8 @@ int llmhip_kv_block_append(llmhip_ctx* ctx, const llmhip_kv_blocks* cache, uint3
  *   slots         device [T], in any order, also the same one twice; < 0: a
  *                 row of zeros. One past the pool gives zeros and is flagged
  *   out_k, out_v  device [T][heads][head_dim] with strides; either may be
- *                 null. Rows that overlap are refused
+ *                 null. Rows that overlap are refused, and outputs in one
+ *                 another's memory unless their strides are the same
  */
 int llmhip_kv_block_read(llmhip_ctx* ctx, const llmhip_kv_blocks* cache, uint32_t dtype, size_t T, const int64_t* slots,
                          void* out_k, int64_t out_k_token, int64_t out_k_head, void* out_v, int64_t out_v_token,

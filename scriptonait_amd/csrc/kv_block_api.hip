@@ -47,6 +47,33 @@ int check_out(const void* p, const int64_t* strides, size_t n, size_t m, uint32_
   return LLMHIP_OK;
 }
 
+// Whether a row of dim values and one of the same array's `from` values on meet:
+// its directions' strides, the largest first, each of which steps past all that the
+// ones behind it span. So only two steps of each can bring them together.
+bool rows_meet(int64_t from, const int64_t* strides, const uint64_t* extents, int n, uint32_t dim) {
+  if (n == 0) return from < (int64_t)dim && from > -(int64_t)dim;
+  if (*extents < 2) return rows_meet(from, strides + 1, extents + 1, n - 1, dim);
+  const int64_t below = from / *strides - (from % *strides < 0);
+  for (int64_t step = below; step <= below + 1; ++step)
+    if ((uint64_t)(step < 0 ? -step : step) < *extents && rows_meet(from - step * *strides, strides + 1, extents + 1, n - 1, dim))
+      return true;
+  return false;
+}
+
+// Whether the rows of two operands, [n][m] of dim values each, are apart: in
+// memory of their own, or of the same strides and beside one another. (Neither's own
+// rows overlap.)
+bool pair_disjoint(const void* p, const void* q, const int64_t (*strides)[2], size_t n, size_t m, uint32_t dim, uint32_t elem) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(p), y = reinterpret_cast<uintptr_t>(q), between = x <= y ? y - x : x - y;
+  const int64_t* low = strides[x <= y ? 0 : 1];
+  if (between >= ((unsigned __int128)(uint64_t)low[0] * (n - 1) + (unsigned __int128)(uint64_t)low[1] * (m - 1) + dim) * elem) return true;
+  if ((n > 1 && strides[0][0] != strides[1][0]) || (m > 1 && strides[0][1] != strides[1][1]) || between % elem) return false;
+  const bool tokens_first = m < 2 || (n > 1 && low[0] >= low[1]);
+  const int64_t ordered[2] = {low[!tokens_first], low[tokens_first]};
+  const uint64_t extents[2] = {tokens_first ? n : m, tokens_first ? m : n};
+  return !rows_meet((int64_t)(between / elem), ordered, extents, 2, dim);
+}
+
 BlockScales scales_of(const llmhip_kv_blocks* c) {
   BlockScales s{};
   s.scale[0] = c->k_scale;
@@ -133,6 +160,8 @@ int llmhip_kv_block_read(llmhip_ctx* ctx, const llmhip_kv_blocks* cache, uint32_
   const int64_t strides[2][2] = {{out_k_token, out_k_head}, {out_v_token, out_v_head}};
   TRY(check_out(out_k, strides[0], T, cache->heads, cache->head_dim, "rows of out_k overlap"));
   TRY(check_out(out_v, strides[1], T, cache->heads, cache->head_dim, "rows of out_v overlap"));
+  ARG(!out_k || !out_v || pair_disjoint(out_k, out_v, strides, T, cache->heads, cache->head_dim, size_of(dtype)),
+      "rows of out_k and out_v overlap");
   ON_DEVICE(info);
   BlockReadArgs a{};
   a.out[0] = out_k;

@@ -26,6 +26,7 @@ CODES = {torch.int8: 4, torch.float8_e4m3fn: 3}
 _ROWS = {t: c for t, c in DTYPES.items() if t is not torch.float8_e4m3fn}
 _i64 = ctypes.c_int64
 MAX_BLOCK, MAX_NEW_TOKENS = 256, 16
+_ERR_ARGUMENT = -1  # LLMHIP_ERR_INVALID_ARGUMENT
 
 
 def _apart(t, inner: int, dims: int) -> bool:
@@ -140,7 +141,8 @@ class BlockKVCache:
     def read(self, slots, out_k=None, out_v=None, stream=None) -> None:
         """llmhip_kv_block_read: the keys and values of the slots ([T] int64;
         negative: a row of zeros) into out_k and out_v [T, heads, head_dim]
-        of float32, bfloat16 or float16; either may be left out."""
+        of float32, bfloat16 or float16; either may be left out. They may be
+        views of one tensor whose rows do not overlap."""
         out = out_k if out_k is not None else out_v
         if out is None:
             raise ValueError("out_k or out_v is required")
@@ -155,6 +157,8 @@ class BlockKVCache:
             *(_NO_ROWS if out_k is None else _out_rows(out_k, shape, dt, "out_k", dev)),
             *(_NO_ROWS if out_v is None else _out_rows(out_v, shape, dt, "out_v", dev)),
             _current(dev) if stream is None else _on(stream, dev, (slots, out_k, out_v, *self._state)))
+        if status == _ERR_ARGUMENT and out_k is not None and out_v is not None:
+            raise ValueError(self.lib.llmhip_last_error().decode(errors="replace"))  # rows of the one over the other's
         if status:
             _check(self.lib, status)
 
