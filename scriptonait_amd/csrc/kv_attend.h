@@ -859,8 +859,11 @@ hipError_t launch_attend_engine(const typename E::Args& a, hipStream_t s) {
     const uint64_t pool = (uint64_t)a.pages * a.page * a.heads * a.dim * E::kElem;
     if constexpr (E::kBlocks) {
       // (Nor where a cache head has more queries than the matrix cores take at once,
-      // whose waves read the same rows: 135 requests of 1656 tokens with 20 for each of
-      // 8 heads of 112 203 us, past the caches 248.)
+      // whose waves read the same rows. 16 calls of 1 to 256 requests with 20 to 128 queries
+      // a cache head, both types of codes, 1 to 12 heads of 64 to 256, pools of 17 to 543
+      // MB: 0.94 of the time past the caches in the mean, 0.79 to 1.03; 135 requests of 1656
+      // tokens with 20 for each of 8 heads of 112 164 us and 196, one of 131072 with 32
+      // for each of 8 heads of 128 82 and 83.)
       const bool once = pool > (64u << 20) && a.blocks == 1u;
       return once ? launch_attend_pages<E, true>(a, s) : launch_attend_pages<E, false>(a, s);
     } else {

@@ -13,8 +13,12 @@
 // of values: 2 * VEC values of a row, VEC pairs, or values that are not rotated.
 //
 // What bounds it: for few tokens the chain slots, rows, maximum, codes (256
-// tokens 7.3 us); for many the traffic, 368 MB of 16384 tokens in 78 us, 4.7 TB/s,
-// of which the vector units are busy for 47.
+// tokens 7.2 us where no block's scale grows); for many the traffic, 368 MB of 16384
+// tokens in 78 us, 4.7 TB/s, of which the vector units are busy for 47. A scale that
+// grows costs a read and a write of its block's kept codes, 8 at a time by the
+// task's lanes one after the other: of 256 single tokens in the middle of their
+// blocks of 16 22 us where all grow, 27 where a fifth do. Prompts, whose blocks begin
+// in the call but for a few, take the same time either way.
 #include <algorithm>
 
 #include "kv_args.h"

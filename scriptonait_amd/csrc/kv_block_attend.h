@@ -9,11 +9,11 @@
 // products: the matrix cores take 16 queries of a cache head at once, whose tokens
 // are read once.
 //
-// What bounds it is reading the cache once: 2.2 GB of 256 requests in 340 us (6.4
-// TB/s; E4M3, which one instruction widens two of, 320), 269 MB of one request in
-// 56 and 7 for the join, as 16 tiles a wave are few for a pipeline to fill. Four
-// new tokens of 64 requests 60 and 10 us (65 with a scale for each token), one 50
-// and 5: partial answers are four times as large, 20 MB written and read.
+// What bounds it is reading the cache once: 2.2 GB of 256 requests in 337-362 us (box
+// to box, E4M3 level; 6.1-6.5 TB/s). Not at that bound: 269 MB of one request in 49
+// to 56 and 7 for the join, with 16 tiles a wave. Four new tokens of 64 requests 63
+// and 10 us (66 with a scale for each token), one 54 and 6: partial answers are
+// four times as large, 20 MB written and read.
 #pragma once
 #include "kv_attend.h"
 
